@@ -9,7 +9,7 @@ from . import _lib, ops, runtime, dp  # noqa: F401
 from ._lib import VlnError, LIB_PATH  # noqa: F401
 from .encoder import EncoderLSTM  # noqa: F401
 from .envdrop_decoder import EnvDropDecoder, Critic  # noqa: F401
-from . import functional, staging, losses, optim, metrics, graphs  # noqa: F401
+from . import functional, staging, losses, vocab, optim, metrics, graphs  # noqa: F401
 from .runtime import DeviceClock  # noqa: F401
 from .graphs import IterationGraph, SegmentedIterationGraph, HandshakeIterationGraph  # noqa: F401
 from .staging import DeviceFeatureStore, PinnedStager, HostBatchFeed  # noqa: F401
@@ -24,5 +24,5 @@ from .decoders import (SoftDotAttention, VisualSoftDotAttention, ActionScoring, 
 __all__ = ["_lib", "ops", "runtime", "dp", "functional", "VlnError", "LIB_PATH", "EncoderLSTM", "EnvDropDecoder",
            "Critic", "SoftDotAttention", "VisualSoftDotAttention", "ActionScoring", "PositionalEncoding", "MLPwithBN",
            "AttnDecoderLSTM", "MonitorDecoder", "SpeakerEncoder", "SpeakerDecoder", "Speaker", "back_translate",
-           "env_drop_mask", "synthetic", "batches", "trainers", "LiveBatch", "LiveSteps", "EnvDropILIteration",
+           "env_drop_mask", "vocab", "synthetic", "batches", "trainers", "LiveBatch", "LiveSteps", "EnvDropILIteration",
            "EnvDropA2CIteration", "SelfMonitorIteration", "FollowerIteration", "SpeakerIteration"]

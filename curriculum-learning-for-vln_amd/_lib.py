@@ -199,6 +199,28 @@ class BnMlpGrads(C.Structure):
                 ("precision", i32), ("bn0_from_wgrad", i32), ("scratch", ptr), ("scratch_floats", i64), ("defer", C.POINTER(ParamJobs))]
 
 
+class Constrain(C.Structure):          # vln_constrain
+    _fields_ = ([(n, ptr) for n in ("in", "out", "logits")] + [(n, i64) for n in ("ld_in", "ld_out", "ld_logits")]
+                + [(n, ptr) for n in ("history", "history_len", "prompt", "prompt_len")] + [("ld_history", i64), ("ld_prompt", i64)]
+                + [(n, ptr) for n in ("repetition", "presence", "frequency", "bias_ids", "bias_values")]
+                + [("ld_bias_ids", i64), ("ld_bias_values", i64), ("allowed", ptr), ("allowed_rows", ptr), ("ld_allowed", i64)]
+                + [(n, f32) for n in ("repetition_all", "presence_all", "frequency_all")]
+                + [(n, i32) for n in ("type", "B", "V", "H", "P", "n_bias", "G", "backward", "pad_")])
+
+
+class Distill(C.Structure):            # vln_distill
+    _fields_ = [("logits", ptr), ("ld", i64), ("ids", ptr), ("ld_ids", i64), ("teacher", ptr), ("ld_teacher", i64), ("teacher_rest", ptr),
+                ("target", ptr), ("ignore_index", i64), ("rows", ptr), ("stats", ptr), ("temperature", f32), ("alpha", f32), ("type", i32),
+                ("teacher_type", i32), ("N", i32), ("V", i32), ("K", i32), ("pad_", i32)]
+
+
+CONSTRAIN_MAX_BIAS = 2048              # VLN_CONSTRAIN_MAX_BIAS
+TOP_LOGITS_MAX = 256                   # VLN_TOP_LOGITS_MAX
+DISTILL_MAX = 256                      # VLN_DISTILL_MAX
+DISTILL_STATS = 12                     # VLN_DISTILL_STATS
+TEMPERATURE_MIN, TEMPERATURE_MAX = 1e-3, 1e3
+REDUCE = {"none": 0, "sum": 1, "mean": 2}
+
 # C struct name -> ctypes mirror: load() compares sizeof on both sides (vln_struct_size)
 STRUCT_MIRRORS = {
     "vln_tick_item": TickItem, "vln_wgrad_job": WgradJob, "vln_colsum_job": ColsumJob, "vln_param_jobs": ParamJobs,
@@ -209,7 +231,7 @@ STRUCT_MIRRORS = {
     "vln_follower_grads": FollowerGrads, "vln_bn_affine": BnAffine, "vln_bn_mlp_layer": BnMlpLayer, "vln_bn_mlp": BnMlp,
     "vln_bn_mlp_grad_layer": BnMlpGradLayer, "vln_bn_mlp_grads": BnMlpGrads, "vln_gather_rollout_step": GatherRolloutStep,
     "vln_gather_ride": GatherRide, "vln_envdrop_dims": EnvDropDims, "vln_envdrop_weights": EnvDropWeights, "vln_envdrop_step": EnvDropStep, "vln_dctx_term": DctxTerm,
-    "vln_envdrop_grads": EnvDropGrads,
+    "vln_envdrop_grads": EnvDropGrads, "vln_constrain": Constrain, "vln_distill": Distill,
 }
 
 # symbol -> (restype, argtypes); must list EVERY function declared in include/vln_hip.h
@@ -273,6 +295,12 @@ SIGNATURES = {
     "vln_monitor_loss_bwd": (i32, [ptr, ptr, ptr, i64, ptr, ptr, ptr, i64, i32, f32, i32, ptr, ptr, i32, i32, i64, ptr]),
     "vln_monitor_loss_multi_fwd": (i32, [C.POINTER(MonitorLossStep), i32, i32, i32, f32, i64, ptr, ptr, i32, ptr]),
     "vln_monitor_loss_multi_bwd": (i32, [C.POINTER(MonitorLossStep), i32, i32, i32, f32, i64, ptr, ptr, ptr]),
+    "vln_constrain_logits": (i32, [C.POINTER(Constrain), ptr]),
+    "vln_top_logits_ws_bytes": (i64, [i32, i32, i32]),
+    "vln_top_logits": (i32, [ptr, i64, i32, i32, i32, i32, f32, ptr, ptr, ptr, ptr, i64, ptr]),
+    "vln_distill_ws_bytes": (i64, [i32, i32, i32]),
+    "vln_distill_fwd": (i32, [C.POINTER(Distill), i32, ptr, ptr, i64, ptr]),
+    "vln_distill_bwd": (i32, [C.POINTER(Distill), ptr, i64, ptr, ptr, i64, ptr]),
     "vln_categorical_fwd": (i32, [ptr, i64, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, u64, u64, ptr, ptr]),
     "vln_categorical_bwd": (i32, [ptr, ptr, ptr, ptr, ptr, i32, i32, ptr]),
     "vln_categorical_multi_bwd": (i32, [C.POINTER(CatStep), i32, i32, ptr, ptr, ptr]),
@@ -363,7 +391,7 @@ SIGNATURES = {
 
 # The ABI this binding was written against (csrc/api.hip::vln_abi_version).  Entry points change their argument lists
 # between versions under the SAME names, so a stale libvln_hip.so must be refused, not called with shifted arguments.
-EXPECTED_ABI = 19
+EXPECTED_ABI = 20
 SHADOW_MAX_JOBS = 24          # include/vln_hip.h VLN_SHADOW_MAX_JOBS
 
 _lib = None

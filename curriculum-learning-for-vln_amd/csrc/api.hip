@@ -118,7 +118,7 @@ extern "C" int vln_prof_read(int kernel_id, int64_t* launches, double* total_ms,
   return VLN_OK;
 }
 
-extern "C" int vln_abi_version(void) { return 19; }
+extern "C" int vln_abi_version(void) { return 20; }
 extern "C" int64_t vln_struct_size(const char* name) {
   if (!name) return -1;
 #define VLN_SZ(T) if (std::strcmp(name, #T) == 0) return (int64_t)sizeof(T)
@@ -153,6 +153,8 @@ extern "C" int64_t vln_struct_size(const char* name) {
   VLN_SZ(vln_envdrop_step);
   VLN_SZ(vln_envdrop_grads);
   VLN_SZ(vln_dctx_term);
+  VLN_SZ(vln_constrain);
+  VLN_SZ(vln_distill);
 #undef VLN_SZ
   return -1;
 }

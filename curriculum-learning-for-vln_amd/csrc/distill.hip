@@ -1,0 +1,463 @@
+// Distillation from a teacher's top logits (vln_distill_fwd / vln_distill_bwd): the loss of a row over the K words the teacher kept,
+// optionally "any other word" as one more outcome, optionally mixed with the cross entropy of a hard target.  include/vln_hip.h states
+// the formulas.
+//
+// Bound: bytes.  The forward reads the logits once (ONE WAVE per row, or per segment of a row when there are few rows: a running
+// (maximum, sum) per lane, joined at the end, no workgroup barrier), the backward reads them again and writes the gradient: nothing of
+// size N x V is kept between the two, only kStat floats per row.  With teacher_rest the sum runs over the words the teacher did NOT
+// keep (a bitmap of the kept ones in LDS, one byte tested per 8 logits): the mass of the others is a sum of positive terms, never
+// 1 - (sum of the kept), which cancels when the student is sure.  The kept words (<= VLN_DISTILL_MAX per row) are handled by their own
+// lanes: loss terms in the forward, and in the backward their gradients overwrite what the streaming loop wrote there.
+#include "word_rows.h"
+#include "../../include/vln_hip.h"
+
+namespace vln {
+
+constexpr int kStat = VLN_DISTILL_STATS;      // per row: see the enum
+enum { ST_FLAGS = 0, ST_M, ST_S, ST_S1, ST_MR, ST_SR, ST_TM, ST_TS, ST_R };
+enum { ROW_LIVE = 1, ROW_SOFT = 2, ROW_TWICE = 4 };      // counted; the teacher has mass; some kept word is listed twice
+
+struct DistillArgs {
+  const void* logits; int64_t ld;
+  const long long* ids; int64_t ld_ids;
+  const void* tvals; int64_t ld_t; int t_bf16;
+  const float* t_rest;
+  const long long* target;
+  long ignore;
+  int N, V, K, S, seg_vecs;
+  float c, invT, T, alpha;
+  float* rows; float* stats;
+  float4* part;               // S > 1: [N, S]
+  // backward
+  void* dz; int64_t ldz; const float* g; long g_stride; const float* inv_count;
+};
+
+__device__ __forceinline__ float teacher_value(const DistillArgs& a, long n, int j) {
+  return a.t_bf16 ? Elt<bf16_raw>::ld(static_cast<const bf16_raw*>(a.tvals) + n * a.ld_t + j)
+                  : static_cast<const float*>(a.tvals)[n * a.ld_t + j];
+}
+// t / T; a finite value stays finite, so that a row masked with the type's lowest value is still a distribution
+__device__ __forceinline__ float teacher_u(const DistillArgs& a, long n, int j) {
+  const float t = teacher_value(a, n, j);
+  return t == -INFINITY ? t : (t < 0.f ? fmaxf(t * a.invT, -FLT_MAX) : t * a.invT);
+}
+__device__ __forceinline__ bool row_ignored(const DistillArgs& a, long n) { return a.target && (long)a.target[n] == a.ignore; }
+
+// Everything of a row that does not need the whole row again, by one wave.  dense / s1: the (maximum, sum) over all words -- or, TAIL,
+// over the words outside `kid` -- at temperature T, and the sum at temperature 1 relative to the same maximum (hard targets).
+// kid [K]: the row's word ids in LDS (-1: absent).
+template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(const DistillArgs& a, long n, OnlineSum dense, float s1, const int* kid,
+                                                                            int lane) {
+  const E* p = static_cast<const E*>(a.logits) + n * a.ld;
+  const float c = a.c;
+  // teacher: maximum and sum over the outcomes present
+  float tm = -INFINITY;
+  bool nan = false;                  // (no maximum takes a NaN: it enters through the sum, and the row's loss is NaN)
+  auto outcome = [&](float u) { tm = fmaxf(tm, u); nan = nan || u != u; };
+  if (TAIL) outcome(a.t_rest[n]);
+  for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) outcome(teacher_u(a, n, j));
+  tm = wave_max(tm);
+  const bool soft = tm != -INFINITY || __any(nan);
+  const float tref = tm != -INFINITY ? tm : 0.f;
+  float ts = 0.f;
+  for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) ts += exp2_hw((teacher_u(a, n, j) - tref) * kLog2e);
+  ts = wave_sum(ts);
+  const float er = TAIL ? exp2_hw((a.t_rest[n] - tref) * kLog2e) : 0.f;
+  ts += er;
+  // a word listed twice: only its first entry counts in the student's total
+  bool twice = false;
+  for (int j = lane; j < a.K; j += 64) {
+    const int id = kid[j];
+    if (id >= 0) for (int i = 0; i < j; ++i) twice = twice || kid[i] == id;
+  }
+  const bool any_twice = __any(twice);
+  // student
+  OnlineSum all = dense;
+  if (TAIL) {
+    float M = dense.m;
+    for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) M = fmaxf(M, Elt<E>::ld(p + kid[j]));
+    M = wave_max(M);
+    float t = 0.f, t1 = 0.f;
+    for (int j = lane; j < a.K; j += 64) {
+      const int id = kid[j];
+      bool first = id >= 0;
+      if (any_twice) for (int i = 0; i < j; ++i) first = first && kid[i] != id;
+      if (first) {
+        const float d = Elt<E>::ld(p + id) - M;
+        t += exp2_hw(d * c);
+        t1 += exp2_hw(d * kLog2e);
+      }
+    }
+    all.s = dense.s * exp2_hw((dense.m - M) * c) + wave_sum(t);
+    s1 = s1 * exp2_hw((dense.m - M) * kLog2e) + wave_sum(t1);
+    all.m = M;
+  }
+  const float log_s = logf(all.s), log_ts = logf(ts);
+  float loss = 0.f;
+  if (soft) {
+    for (int j = lane; j < a.K; j += 64) {
+      const int id = kid[j];
+      if (id < 0) continue;
+      const float lq = (teacher_u(a, n, j) - tref) - log_ts, q = exp2_hw(lq * kLog2e);
+      const float z = Elt<E>::ld(p + id);
+      const float lp = z == -INFINITY ? -INFINITY : (z - all.m) * a.invT - log_s;
+      if (q != 0.f) loss += q * (lq - lp);
+    }
+    if (TAIL && lane == 0 && er != 0.f) {
+      const float lr = (a.t_rest[n] - tref) - log_ts;
+      const float lpr = dense.s == 0.f ? -INFINITY : (dense.m - all.m) * a.invT + logf(dense.s) - log_s;
+      loss += exp2_hw(lr * kLog2e) * (lr - lpr);
+    }
+  }
+  loss = wave_sum(loss) * a.alpha * a.T * a.T;
+  if (a.alpha == 0.f) loss = 0.f;
+  const bool live = a.target ? !row_ignored(a, n) : soft;
+  if (a.target && a.alpha < 1.f) {
+    const long y = (long)a.target[n];
+    const float z = (y >= 0 && y < a.V) ? Elt<E>::ld(p + y) : __builtin_nanf("");
+    loss += (1.f - a.alpha) * (all.m - z + logf(s1));
+  }
+  if (lane == 0) {
+    a.rows[n] = live ? loss : 0.f;
+    float* st = a.stats + n * kStat;
+    st[ST_FLAGS] = __int_as_float((live ? ROW_LIVE : 0) | (soft ? ROW_SOFT : 0) | (any_twice ? ROW_TWICE : 0));
+    st[ST_M] = all.m; st[ST_S] = all.s; st[ST_S1] = s1;
+    st[ST_MR] = dense.m; st[ST_SR] = dense.s;
+    st[ST_TM] = tref; st[ST_TS] = ts;
+    st[ST_R] = soft ? er / ts : 0.f;
+  }
+}
+__device__ __forceinline__ void dead_row(const DistillArgs& a, long n, int lane) {
+  if (lane == 0) { a.rows[n] = 0.f; a.stats[n * kStat + ST_FLAGS] = __int_as_float(0); }
+}
+__device__ __forceinline__ void stage_ids(const DistillArgs& a, long n, int* kid, int lane) {
+  for (int j = lane; j < a.K; j += 64) {
+    const long long id = a.ids[n * a.ld_ids + j];
+    kid[j] = (id >= 0 && id < a.V) ? (int)id : -1;
+  }
+  __syncthreads();
+}
+
+// HARD: also the sum at temperature 1 (T != 1 and a hard target); otherwise s1 is the sum at T.
+template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) void distill_fwd_kernel(DistillArgs a) {
+  extern __shared__ unsigned lds[];
+  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC;
+  const long n = blockIdx.x;
+  const int s = blockIdx.y, lane = threadIdx.x;
+  if (row_ignored(a, n)) { if (s == 0) dead_row(a, n, lane); return; }
+  const E* p = static_cast<const E*>(a.logits) + n * a.ld;
+  const RowGeo<E> g(p, a.V);
+  const int v0 = min(g.nv, s * a.seg_vecs), v1 = min(g.nv, v0 + a.seg_vecs);
+  int* kid = reinterpret_cast<int*>(lds);
+  unsigned* bm = lds + (a.K + 3) / 4 * 4;        // bit i: column i of the segment's vectors; then head, then tail (VEC bits each)
+  const int nbits_v = a.seg_vecs * VEC;
+  if (TAIL || a.S == 1) stage_ids(a, n, kid, lane);
+  if (TAIL) {
+    const int nw = (nbits_v + 2 * VEC + 31) / 32;
+    for (int i = lane; i < nw; i += 64) bm[i] = 0u;
+    __syncthreads();
+    for (int j = lane; j < a.K; j += 64) {
+      const int id = kid[j];
+      if (id < 0) continue;
+      int bit = -1;
+      if (id < g.head) bit = nbits_v + id;
+      else if (id >= g.tail0()) bit = nbits_v + VEC + (id - g.tail0());
+      else { const int i = id - g.head - v0 * VEC; if (i >= 0 && i < (v1 - v0) * VEC) bit = i; }
+      if (bit >= 0) atomicOr(&bm[bit >> 5], 1u << (bit & 31));
+    }
+    __syncthreads();
+  }
+  OnlineSum o;
+  float s1 = 0.f;
+  auto take = [&](const auto& x, float mx) {
+    constexpr int N = sizeof(x) / sizeof(float);
+    if (mx > o.m) {
+      if (HARD) s1 *= exp2_hw((o.m - mx) * kLog2e);
+      o.raise(mx, a.c);
+    }
+    float t = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = x[i] - o.m;
+      t += exp2_hw(d * a.c);
+      if (HARD) t1 += exp2_hw(d * kLog2e);
+    }
+    o.s += t;
+    if (HARD) s1 += t1;
+  };
+  if (s == 0) {
+    int col = -1, bit = 0;
+    if (lane < g.head) { col = lane; bit = nbits_v + lane; }
+    else if (lane >= VEC && lane - VEC < g.tail) { col = g.tail0() + lane - VEC; bit = nbits_v + lane; }
+    float x[1] = {col >= 0 ? Elt<E>::ld(p + col) : -INFINITY};
+    if (TAIL && col >= 0 && ((bm[bit >> 5] >> (bit & 31)) & 1u)) x[0] = -INFINITY;
+    take(x, x[0]);
+  }
+  for (int v = v0 + lane; v < v1; v += 64 * U) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * 64, v1 - 1) * VEC);
+    float x[16];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unpack16<E>(raw[u], x + u * VEC);
+      unsigned out = 0u;             // bit j: element j does not count
+      if (TAIL) { const int bit = (v + u * 64 - v0) * VEC; if (v + u * 64 < v1) out = (bm[bit >> 5] >> (bit & 31)) & ((1u << VEC) - 1u); }
+      if (v + u * 64 >= v1) out = ~0u;
+      if (out) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) if ((out >> j) & 1u) x[u * VEC + j] = -INFINITY;
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) mx = fmaxf(mx, x[j]);
+    take(x, mx);
+  }
+  // the wave's total
+  const float M = wave_max(o.m);
+  if (HARD) s1 = wave_sum(s1 * exp2_hw((o.m - M) * kLog2e));
+  o.s = wave_sum(o.s * exp2_hw((o.m - M) * a.c));
+  o.m = M;
+  if (!HARD) s1 = o.s;
+  if (a.S == 1) finish_row<E, TAIL>(a, n, o, s1, kid, lane);
+  else if (lane == 0) a.part[n * a.S + s] = make_float4(o.m, o.s, s1, 0.f);
+}
+
+template <typename E, bool TAIL> __global__ __launch_bounds__(64) void distill_join_kernel(DistillArgs a) {
+  extern __shared__ unsigned lds[];
+  const long n = blockIdx.x;
+  const int lane = threadIdx.x;
+  if (row_ignored(a, n)) return;
+  int* kid = reinterpret_cast<int*>(lds);
+  stage_ids(a, n, kid, lane);
+  OnlineSum o;
+  float s1 = 0.f;
+  for (int i = lane; i < a.S; i += 64) {
+    const float4 q = a.part[n * a.S + i];
+    const float M = fmaxf(o.m, q.x);
+    s1 = s1 * exp2_hw((o.m - M) * kLog2e) + q.z * exp2_hw((q.x - M) * kLog2e);
+    o.merge(q.x, q.y, a.c);
+  }
+  const float M = wave_max(o.m);
+  s1 = wave_sum(s1 * exp2_hw((o.m - M) * kLog2e));
+  o.wave(a.c);
+  finish_row<E, TAIL>(a, n, o, s1, kid, lane);
+}
+
+// sum or mean over the rows, in a fixed order: out[0] = loss, out[1] = what the backward multiplies every row's gradient with
+__global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows, const float* stats, int N, int mean, float* out) {
+  __shared__ float part[16];
+  __shared__ int cnt[16];
+  float acc = 0.f;
+  int n = 0;
+  for (int i = threadIdx.x; i < N; i += 1024) {
+    acc += rows[i];
+    n += __float_as_int(stats[(long)i * kStat + ST_FLAGS]) & ROW_LIVE;
+  }
+  acc = wave_sum(acc);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = acc; cnt[threadIdx.x >> 6] = n; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    int c = 0;
+    for (int i = 0; i < 16; ++i) { t += part[i]; c += cnt[i]; }
+    out[0] = mean ? t / (float)c : t;
+    out[1] = mean ? 1.f / (float)c : 1.f;
+  }
+}
+
+// d z_v = g [ alpha T (p_v - q_v) + (1 - alpha) (softmax(z)_v - [v = y]) ], p_v - r p_v / p_rest for the words the teacher did not keep.
+// The streaming loop evaluates  A exp((z - M) / T) + H exp(z - M)  with one pair (A, H) per row: M is the maximum the exponentials of
+// that loop are bounded by (TAIL: the others' maximum), so neither a sure student's tiny p_rest nor its kept words leave the range.
+template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) void distill_bwd_kernel(DistillArgs a) {
+  extern __shared__ unsigned lds[];
+  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC;
+  const long n = blockIdx.x;
+  const int s = blockIdx.y, lane = threadIdx.x;
+  const E* p = static_cast<const E*>(a.logits) + n * a.ld;
+  E* dz = static_cast<E*>(a.dz) + n * a.ldz;
+  const float* st = a.stats + n * kStat;
+  const int flags = __float_as_int(st[ST_FLAGS]);
+  const RowGeo<E> g(dz, a.V);                 // the writes decide the alignment
+  const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
+  const int v0 = min(g.nv, s * a.seg_vecs), v1 = min(g.nv, v0 + a.seg_vecs);
+  const bool single = s == 0 && (lane < g.head || (lane >= VEC && lane - VEC < g.tail));
+  const int scol = lane < g.head ? lane : g.tail0() + lane - VEC;
+  if (!(flags & ROW_LIVE)) {                  // an ignored row: zeros, whatever its logits hold
+    if (single) Elt<E>::st(dz + scol, 0.f);
+    for (int v = v0 + lane; v < v1; v += 64) st_vec<E>(dz + g.head + (int64_t)v * VEC, make_uint4(0, 0, 0, 0));
+    return;
+  }
+  const float up = a.g[n * a.g_stride] * (a.inv_count ? a.inv_count[0] : 1.f);
+  const bool soft = (flags & ROW_SOFT) != 0 && a.alpha != 0.f;
+  const float m = st[ST_M], sum = st[ST_S], s1 = st[ST_S1], r = TAIL ? st[ST_R] : 0.f;
+  const float M = TAIL ? st[ST_MR] : m, sr = st[ST_SR];
+  const float gs = soft ? up * a.alpha * a.T : 0.f;                  // soft term's factor
+  const bool hard = a.target != nullptr && a.alpha < 1.f;
+  const float gh = hard ? up * (1.f - a.alpha) : 0.f;
+  const float is = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum), is1 = s1 > 0.f ? 1.f / s1 : (s1 == 0.f ? 0.f : s1);
+  float A = gs * (exp2_hw((M - m) * a.c) * is - (TAIL && sr > 0.f ? r / sr : 0.f));
+  float H = gh * exp2_hw((M - m) * kLog2e) * is1;
+  const long y = hard ? (long)a.target[n] : -1;
+  const bool bad_y = hard && (y < 0 || y >= a.V);
+  if (bad_y) H = __builtin_nanf("");
+  if (!HARD) A += H;                          // temperature 1: one exponential serves both terms
+  auto grad = [&](float z) {
+    const float d = z - M;
+    float v = A * exp2_hw(d * a.c);
+    if (HARD) v += H * exp2_hw(d * kLog2e);
+    return v;
+  };
+  if (single) Elt<E>::st(dz + scol, grad(Elt<E>::ld(p + scol)));
+  if (same) {
+    for (int v = v0 + lane; v < v1; v += 64 * U) {
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * 64, v1 - 1) * VEC);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[VEC];
+        unpack16<E>(raw[u], x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = grad(x[j]);
+        if (v + u * 64 < v1) st_vec<E>(dz + g.head + (int64_t)(v + u * 64) * VEC, pack16<E>(x));
+      }
+    }
+  } else {                                    // rows that start at different distances from a 16-byte boundary
+    for (int c = g.head + v0 * VEC + lane; c < g.head + v1 * VEC; c += 64) Elt<E>::st(dz + c, grad(Elt<E>::ld(p + c)));
+  }
+  // the kept words and the target: their own values over what the loop wrote
+  int* kid = reinterpret_cast<int*>(lds);
+  const int nk = soft || TAIL ? a.K : 0;
+  if (nk) stage_ids(a, n, kid, lane); else __syncthreads();
+  auto mine = [&](long id) {
+    if (id < g.head || id >= g.tail0()) return s == 0;
+    const int i = (int)((id - g.head) / VEC);
+    return i >= v0 && i < v1;
+  };
+  const float tm = st[ST_TM], its = 1.f / st[ST_TS];
+  auto kept = [&](int id, float q) {          // gradient of a word with the teacher's probability q
+    const float d = Elt<E>::ld(p + id) - m;
+    float v = gs * (exp2_hw(d * a.c) * is - q);
+    if (hard) v += gh * (exp2_hw(d * kLog2e) * is1 - (id == y ? 1.f : 0.f));
+    return bad_y ? __builtin_nanf("") : v;
+  };
+  bool y_kept = false;
+  for (int j = lane; j < nk; j += 64) {
+    const int id = kid[j];
+    if (id < 0) continue;
+    y_kept = y_kept || id == y;
+    if (!mine(id)) continue;
+    float q = soft ? exp2_hw((teacher_u(a, n, j) - tm) * kLog2e) * its : 0.f;
+    if (soft && (flags & ROW_TWICE)) {                  // listed more than once: the first entry writes the sum, in entry order
+      bool first = true;
+      for (int i = 0; i < j; ++i) first = first && kid[i] != id;
+      if (!first) continue;
+      for (int i = j + 1; i < a.K; ++i) if (kid[i] == id) q += exp2_hw((teacher_u(a, n, i) - tm) * kLog2e) * its;
+    }
+    Elt<E>::st(dz + id, kept(id, q));
+  }
+  if (hard && !bad_y && !__any(y_kept) && lane == 0 && mine(y)) {
+    Elt<E>::st(dz + y, grad(Elt<E>::ld(p + y)) - gh);
+  }
+}
+
+// Segments per row: 32 waves per CU when every row is one wave; with fewer rows split, but no segment under four rounds of the wave's loads
+static void distill_split(int N, int V, int vec, int* S, int* seg_vecs) {
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  const int nv = (V + vec - 1) / vec;
+  const int want = (16 * cus + N - 1) / N, most = (nv + 511) / 512;
+  int n = want < most ? want : most;
+  const int least = (nv + 32767) / 32768;                     // (a segment's bitmap stays at 32 KB of LDS)
+  if (n < least) n = least;
+  if (n < 1) n = 1;
+  *seg_vecs = ((nv + n - 1) / n + 63) / 64 * 64;
+  *S = (nv + *seg_vecs - 1) / *seg_vecs;
+}
+
+template <typename E, bool TAIL> static int distill_fwd_launch(const DistillArgs& a, bool hard, int reduce, float* out, hipStream_t st) {
+  const unsigned ids = (unsigned)((a.K + 3) / 4 * 16);
+  const unsigned bits = TAIL ? (unsigned)((a.seg_vecs * Elt<E>::kVec + 2 * Elt<E>::kVec + 31) / 32 * 4) : 0u;
+  const dim3 grid((unsigned)a.N, (unsigned)a.S);
+  if (hard) VLN_LAUNCH((distill_fwd_kernel<E, TAIL, true>), grid, dim3(64), ids + bits, st, a);
+  else VLN_LAUNCH((distill_fwd_kernel<E, TAIL, false>), grid, dim3(64), ids + bits, st, a);
+  if (a.S > 1) VLN_LAUNCH((distill_join_kernel<E, TAIL>), dim3((unsigned)a.N), dim3(64), ids, st, a);
+  if (reduce) VLN_LAUNCH(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, (const float*)a.rows, (const float*)a.stats, a.N, reduce == VLN_REDUCE_MEAN ? 1 : 0, out);
+  VLN_CHECK_LAUNCH("distill_fwd");
+  return VLN_OK;
+}
+template <typename E, bool TAIL> static int distill_bwd_launch(const DistillArgs& a, bool hard, hipStream_t st) {
+  const dim3 grid((unsigned)a.N, (unsigned)a.S);
+  const unsigned ids = (unsigned)((a.K + 3) / 4 * 16);
+  if (hard) VLN_LAUNCH((distill_bwd_kernel<E, TAIL, true>), grid, dim3(64), ids, st, a);
+  else VLN_LAUNCH((distill_bwd_kernel<E, TAIL, false>), grid, dim3(64), ids, st, a);
+  VLN_CHECK_LAUNCH("distill_bwd");
+  return VLN_OK;
+}
+
+static int distill_args(const vln_distill* p, DistillArgs& a, const char* who) {
+  if (!p) { set_error("%s: null pointer", who); return VLN_ERR_ARG; }
+  if (p->N <= 0 || p->V <= 0 || !p->logits || p->ld < p->V) { set_error("%s: bad logits", who); return VLN_ERR_ARG; }
+  if (p->K < 1 || p->K > VLN_DISTILL_MAX || !p->ids || !p->teacher || p->ld_ids < p->K || p->ld_teacher < p->K) {
+    set_error("%s: the teacher keeps 1 .. %d words per row", who, VLN_DISTILL_MAX); return VLN_ERR_ARG;
+  }
+  if ((p->type != VLN_F32 && p->type != VLN_BF16) || (p->teacher_type != VLN_F32 && p->teacher_type != VLN_BF16)) {
+    set_error("%s: types must be fp32 or bf16", who); return VLN_ERR_ARG;
+  }
+  if (!(p->temperature >= VLN_TEMPERATURE_MIN && p->temperature <= VLN_TEMPERATURE_MAX) || !(p->alpha >= 0.f && p->alpha <= 1.f)) {
+    set_error("%s: bad temperature / alpha", who); return VLN_ERR_ARG;
+  }
+  if (p->alpha < 1.f && !p->target) { set_error("%s: alpha < 1 needs hard targets", who); return VLN_ERR_ARG; }
+  if (!p->rows || !p->stats) { set_error("%s: rows / stats missing", who); return VLN_ERR_ARG; }
+  a = DistillArgs{};
+  a.logits = p->logits; a.ld = p->ld;
+  a.ids = (const long long*)p->ids; a.ld_ids = p->ld_ids;
+  a.tvals = p->teacher; a.ld_t = p->ld_teacher; a.t_bf16 = p->teacher_type == VLN_BF16;
+  a.t_rest = p->teacher_rest;
+  a.target = (const long long*)p->target; a.ignore = (long)p->ignore_index;
+  a.N = p->N; a.V = p->V; a.K = p->K;
+  a.c = kLog2e / p->temperature; a.invT = 1.f / p->temperature; a.T = p->temperature; a.alpha = p->alpha;
+  a.rows = p->rows; a.stats = p->stats;
+  distill_split(a.N, a.V, p->type == VLN_F32 ? 4 : 8, &a.S, &a.seg_vecs);
+  return VLN_OK;
+}
+
+}  // namespace vln
+
+extern "C" int64_t vln_distill_ws_bytes(int N, int V, int type) {
+  if (N <= 0 || V <= 0 || (type != VLN_F32 && type != VLN_BF16)) return 0;
+  int S, sv;
+  vln::distill_split(N, V, type == VLN_F32 ? 4 : 8, &S, &sv);
+  return S > 1 ? (int64_t)N * S * 16 : 0;
+}
+extern "C" int vln_distill_fwd(const vln_distill* p, int reduction, float* out, void* ws, int64_t ws_bytes, vln_stream_t s) {
+  vln::DistillArgs a;
+  const int rc = vln::distill_args(p, a, "vln_distill_fwd");
+  if (rc != VLN_OK) return rc;
+  if ((reduction != VLN_REDUCE_NONE && reduction != VLN_REDUCE_SUM && reduction != VLN_REDUCE_MEAN) || (reduction != VLN_REDUCE_NONE && !out)) {
+    vln::set_error("vln_distill_fwd: bad reduction"); return VLN_ERR_ARG;
+  }
+  if (a.S > 1) {
+    if (!ws || ws_bytes < (int64_t)a.N * a.S * 16) { vln::set_error("vln_distill_fwd: workspace too small"); return VLN_ERR_ARG; }
+    a.part = static_cast<float4*>(ws);
+  }
+  const bool hard = a.alpha < 1.f && a.T != 1.f;
+  hipStream_t st = (hipStream_t)s;
+  if (p->type == VLN_F32) return a.t_rest ? vln::distill_fwd_launch<float, true>(a, hard, reduction, out, st) : vln::distill_fwd_launch<float, false>(a, hard, reduction, out, st);
+  return a.t_rest ? vln::distill_fwd_launch<bf16_raw, true>(a, hard, reduction, out, st) : vln::distill_fwd_launch<bf16_raw, false>(a, hard, reduction, out, st);
+}
+extern "C" int vln_distill_bwd(const vln_distill* p, const float* dloss, int64_t dloss_stride, const float* inv_count, void* dlogits, int64_t ld_dlogits,
+                               vln_stream_t s) {
+  vln::DistillArgs a;
+  const int rc = vln::distill_args(p, a, "vln_distill_bwd");
+  if (rc != VLN_OK) return rc;
+  if (!dloss || (dloss_stride != 0 && dloss_stride != 1) || !dlogits || ld_dlogits < p->V) { vln::set_error("vln_distill_bwd: bad args"); return VLN_ERR_ARG; }
+  a.g = dloss; a.g_stride = (long)dloss_stride; a.inv_count = inv_count; a.dz = dlogits; a.ldz = ld_dlogits;
+  const bool hard = a.alpha < 1.f && a.T != 1.f;
+  hipStream_t st = (hipStream_t)s;
+  if (p->type == VLN_F32) return a.t_rest ? vln::distill_bwd_launch<float, true>(a, hard, st) : vln::distill_bwd_launch<float, false>(a, hard, st);
+  return a.t_rest ? vln::distill_bwd_launch<bf16_raw, true>(a, hard, st) : vln::distill_bwd_launch<bf16_raw, false>(a, hard, st);
+}

@@ -42,7 +42,7 @@ typedef void* vln_stream_t; /* hipStream_t */
 #define VLN_ACT_RELU 2
 #define VLN_ACT_ACCUM 8   /* flag, OR-ed onto an activation: the finished result is ADDED to the output (vln_linear_fwd: Y += ...) */
 
-int vln_abi_version(void);     /* 19 */
+int vln_abi_version(void);     /* 20 */
 /* sizeof(struct vln_<name>) as THIS library was compiled, -1 for an unknown name: a binding checks its struct mirrors against
  * it when it loads the library (a mirror that is one field short makes the kernels read wild pointers). */
 int64_t vln_struct_size(const char* name);
@@ -339,6 +339,79 @@ int vln_masked_ce_mean_fwd(float* logits, int64_t ld, const int64_t* target, con
                            float* probs /*[B,C]*/, int B, int C, int64_t ignore_index, float* rows_scratch, vln_stream_t s);
 int vln_masked_ce_mean_bwd(const float* probs, const int64_t* target, const float* dloss /*[1]*/, const float* inv_count /*mean_out + 1*/,
                            float* dlogits, int B, int C, int64_t ignore_index, vln_stream_t s);
+
+/* ---- word logits (ABI v20): what a word head answers with and learns from.  Logits [N, V] fp32 or bf16 (`type`), rows `ld` elements
+ * apart (any alignment), arithmetic in fp32, ONE rounding to the logits' type at the end.  No atomics on floats: same inputs, same bits. */
+
+/* Constraints on the logits before a word is drawn (speaker.py:336 bans <UNK> this way; the rest the reference does not have):
+ *   c_v = times v stands in history[b, : history_len[b]];  seen_v = c_v > 0 or v stands in prompt[b, : prompt_len[b]]
+ *   t = z_v;  if (seen_v) t = t > 0 ? t / repetition_b : t * repetition_b
+ *   if (c_v > 0) t -= frequency_b * c_v + presence_b;   t += sum of bias_values[b, j] over the entries j with bias_ids[b, j] == v
+ *   out_v = allowed(b, v) ? t : -inf
+ * Ids outside [0, V) (padding: -1) stand for no word.  allowed: packed bits, word v of mask row r = bit v % 32 of
+ * allowed[r * ld_allowed + v / 32], 1 = allowed; the row's mask row is allowed_rows[b] (-1: every word allowed; outside [-1, G): none),
+ * without allowed_rows it is b (G == B) or 0 (G == 1).  out may be `in` itself (same stride), otherwise they must not overlap.
+ * backward != 0: in = d out, out = d logits (may be the same array), `logits` = the forward's input; biases and penalties get no gradient.
+ * repetition / presence / frequency: [B], or NULL and the *_all value. */
+typedef struct vln_constrain {
+  const void* in; void* out; const void* logits;
+  int64_t ld_in, ld_out, ld_logits;
+  const int64_t* history; const int64_t* history_len; const int64_t* prompt; const int64_t* prompt_len;
+  int64_t ld_history, ld_prompt;
+  const float* repetition; const float* presence; const float* frequency;
+  const int64_t* bias_ids; const float* bias_values;
+  int64_t ld_bias_ids, ld_bias_values;
+  const int32_t* allowed; const int64_t* allowed_rows;
+  int64_t ld_allowed;
+  float repetition_all, presence_all, frequency_all;
+  int32_t type, B, V, H, P, n_bias, G, backward;
+  int32_t pad_;
+} vln_constrain;
+#define VLN_CONSTRAIN_MAX_BIAS 2048
+int vln_constrain_logits(const vln_constrain* args, vln_stream_t s);
+
+/* The k largest logits of every row, largest first, equal values in index order (NaN counts as largest): values [N, k] in the logits'
+ * type, ids [N, k]; rest [N] = log sum over all OTHER words of exp(z / temperature) (-inf: none) -- what vln_distill takes as
+ * `teacher_rest`.  k <= VLN_TOP_LOGITS_MAX.  ws: vln_top_logits_ws_bytes (0: may be NULL). */
+#define VLN_TOP_LOGITS_MAX 256
+#define VLN_TEMPERATURE_MIN 1e-3f
+#define VLN_TEMPERATURE_MAX 1e3f
+int64_t vln_top_logits_ws_bytes(int N, int V, int k);
+int vln_top_logits(const void* logits, int64_t ld, int type, int N, int V, int k, float temperature, void* values, int64_t* ids,
+                   float* rest, void* ws, int64_t ws_bytes, vln_stream_t s);
+
+/* Distillation from a teacher that kept K words per row: ids [N, K] (outside [0, V): absent), their logits `teacher` [N, K], and
+ * optionally teacher_rest [N], the log-mass of all other words at `temperature` (NULL: none -- the teacher is renormalised over the K).
+ *   q_j = exp(t_j / T) / Z, r = exp(rest) / Z, Z = their sum;  p = softmax(z / T), p_rest = the sum of p over words that are not kept
+ *   soft = sum_j q_j (log q_j - log p_{id_j}) + r (log r - log p_rest)
+ *   row  = alpha T^2 soft + (1 - alpha) (log sum exp(z) - z_target)
+ *   d row / d z_v = alpha T (p_v - sum of q_j with id_j = v)  for a kept word,  alpha T (p_v - r p_v / p_rest)  for any other,
+ *                   + (1 - alpha) (softmax(z)_v - [v = target])
+ * A word listed twice: two outcomes that share a word.  A row whose target is ignore_index -- without targets, a row whose teacher has
+ * no mass -- has loss 0 and gradient 0 and is not counted by the mean (no row counted: NaN); any other target outside [0, V) makes its
+ * row NaN.  With targets, a row whose teacher has no mass keeps its hard term.  alpha < 1 needs targets.
+ * rows [N] receives the row losses, stats [N, VLN_DISTILL_STATS] what the backward needs, out[0] the loss and out[1] the factor that the
+ * backward takes as inv_count (reduction != VLN_REDUCE_NONE).  ws: vln_distill_ws_bytes (0: may be NULL). */
+#define VLN_DISTILL_MAX 256
+#define VLN_DISTILL_STATS 12
+#define VLN_REDUCE_NONE 0
+#define VLN_REDUCE_SUM 1
+#define VLN_REDUCE_MEAN 2
+typedef struct vln_distill {
+  const void* logits; int64_t ld;
+  const int64_t* ids; int64_t ld_ids;
+  const void* teacher; int64_t ld_teacher;
+  const float* teacher_rest; const int64_t* target;
+  int64_t ignore_index;
+  float* rows; float* stats;
+  float temperature, alpha;
+  int32_t type, teacher_type, N, V, K, pad_;
+} vln_distill;
+int64_t vln_distill_ws_bytes(int N, int V, int type);
+int vln_distill_fwd(const vln_distill* args, int reduction, float* out, void* ws, int64_t ws_bytes, vln_stream_t s);
+/* dloss_stride 1: one upstream gradient per row, 0: one for all; inv_count: the forward's out + 1 (NULL: 1) */
+int vln_distill_bwd(const vln_distill* args, const float* dloss, int64_t dloss_stride, const float* inv_count, void* dlogits,
+                    int64_t ld_dlogits, vln_stream_t s);
 
 /* The IL loss of a WHOLE rollout, ml_loss = sum_t CrossEntropy(mask(logits_t), target_t) (envdrop.py:173-179 summed over
  * the steps), in one launch after the last decoder step, and all the d logits_t in one launch at the start of backward:
