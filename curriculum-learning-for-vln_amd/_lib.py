@@ -296,7 +296,7 @@ SIGNATURES = {
     "vln_monitor_loss_multi_fwd": (i32, [C.POINTER(MonitorLossStep), i32, i32, i32, f32, i64, ptr, ptr, i32, ptr]),
     "vln_monitor_loss_multi_bwd": (i32, [C.POINTER(MonitorLossStep), i32, i32, i32, f32, i64, ptr, ptr, ptr]),
     "vln_constrain_logits": (i32, [C.POINTER(Constrain), ptr]),
-    "vln_top_logits_ws_bytes": (i64, [i32, i32, i32]),
+    "vln_top_logits_ws_bytes": (i64, [i32, i32, i32, i32]),
     "vln_top_logits": (i32, [ptr, i64, i32, i32, i32, i32, f32, ptr, ptr, ptr, ptr, i64, ptr]),
     "vln_distill_ws_bytes": (i64, [i32, i32, i32]),
     "vln_distill_fwd": (i32, [C.POINTER(Distill), i32, ptr, ptr, i64, ptr]),

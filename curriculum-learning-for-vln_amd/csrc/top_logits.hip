@@ -1,16 +1,16 @@
 // The k largest logits of every row, sorted, and the log-mass of all others (vln_top_logits): a teacher's targets for vln_distill_*,
 // and with k = 1 the greedy word.  include/vln_hip.h states the contract.
 //
-// Bound: bytes (the row is read once) for many rows; latency of one wave's chain for few.  ONE WAVE streams a row (or, with few
-// rows, one of S segments of it) in chunks of 16 elements per lane and keeps the candidates in a small LDS buffer: no workgroup
-// barrier anywhere.  Elements are compared as 64-bit keys (order-preserving bits of the value, complement of the index), all
-// distinct, so ties fall to the lowest index and the result does not depend on the order in which candidates were collected.
-//   * the first chunk's threshold is the k-th largest of the lanes' maxima (found bit by bit with ballots): at least k elements
-//     reach it, and at most 16 k / (maxima per lane) do;
-//   * afterwards an element enters the buffer only above the k-th best key so far; a full buffer is cut back to its k best;
-//   * everything that is not kept goes into the running (maximum, sum) of exp(z / T), also what a cut throws out, so that the
-//     others' mass is a sum of positive terms and never a difference.
-// Segments leave k sorted keys each and a second launch merges them with the same buffer.
+// Bound: bytes for many rows (the row is read once, into registers: all its loads are in flight at once), the length of one workgroup's
+// chain for few.  A workgroup of W waves holds a row, or one of S segments of it, as NVR vectors of 16 bytes per thread:
+//   1. the largest element of every thread (G groups per thread, so that there are >= 4 k groups): at least k elements reach the k-th
+//      largest of these group maxima, and hardly more than k do -- a bound that costs a bisection over 64 W G numbers;
+//   2. one sweep over the registers: elements above the bound are candidates (an LDS list), all others go into the running (maximum,
+//      sum) of exp(z / T) -- the others' mass is a sum of positive terms, never a difference;
+//   3. a candidate's place is the number of larger ones; places from k on belong to the others.
+// Elements are ordered by (order-preserving bits of the value, lower index first): all distinct, so ties fall to the lowest index and the
+// order in which candidates were collected does not show.  Where more reach the bound than the list holds (constant or masked rows), the
+// exact border is found by bisection over value and index.  Segments leave their k best, and one workgroup per row selects among them.
 #include "word_rows.h"
 #include "../../include/vln_hip.h"
 
@@ -18,314 +18,396 @@ namespace vln {
 
 typedef unsigned long long u64;
 
-// value <-> order-preserving bits; every NaN is the largest, -0 equals +0.  0 is no element's key.
+// value <-> order-preserving bits; every NaN is the largest, -0 equals +0.  0 is no element's.
 __device__ __forceinline__ unsigned order_bits(float x) {
   const unsigned b = __float_as_uint(x + 0.f);
-  if (x != x) return 0xffffffffu;
-  return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+  return x != x ? 0xffffffffu : b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float order_value(unsigned o) {
   if (o == 0xffffffffu) return __builtin_nanf("");
   return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
 }
-__device__ __forceinline__ u64 make_key(float x, unsigned idx) { return ((u64)order_bits(x) << 32) | (u64)(~idx); }
 
 struct TopArgs {
   const void* logits; int64_t ld;
-  int N, V, k, S, seg;             // seg: elements per segment (a multiple of the chunk), S segments per row
+  int N, V, k, S;                  // S segments per row
   float c, invT;                   // log2(e) / T, 1 / T
   void* values; long long* ids; float* rest;
-  u64* keys; float2* sums;         // S > 1: [N, S, k] and [N, S]
+  u64* keys; float2* sums;         // S > 1: [N, S, k] (order bits << 32 | ~index; 0: none) and [N, S]
 };
 
 __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // NaN wins (v_maximum3_f32)
 
-// A wave's candidates.  KB: k <= KB; NK registers per lane hold the whole buffer while it is cut.
-template <int KB> struct Candidates {
-  static constexpr int CAP = 2 * KB + 64, NK = CAP / 64;
-  u64* buf;              // [CAP] LDS of this wave
-  int cnt, k;
-  u64 tkey;              // keys above it may enter
-  float tval;            // an element with !(x <= tval) may be above tkey (NaN: all)
-  OnlineSum others;      // per lane
-  float c;
-  int lane;
-
-  __device__ __forceinline__ void init(u64* b, int k_, float c_, int lane_) {
-    buf = b; cnt = 0; k = k_; tkey = 0; tval = __builtin_nanf(""); c = c_; lane = lane_;
-  }
-  // cut the buffer to its k best (call with cnt > k)
-  __device__ __forceinline__ void cut() {
-    unsigned hi[NK], lo[NK];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int at = i * 64 + lane;
-      const u64 v = at < cnt ? buf[at] : 0;
-      hi[i] = (unsigned)(v >> 32); lo[i] = (unsigned)v;
-    }
-    // the largest th with at least k keys of hi >= th, bit by bit; the search ends early where exactly k reach it
-    unsigned th = 0, tl = 0;
-    bool exact = false;
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned t = th | (1u << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < NK; ++i) n += __popcll(__ballot(hi[i] >= t));
-      if (n >= k) { th = t; if (n == k) { exact = true; break; } }
-    }
-    if (!exact) {          // equal values at the border: of those, the `need` lowest indices (largest lo)
-      int need = k;
-#pragma unroll
-      for (int i = 0; i < NK; ++i) need -= __popcll(__ballot(hi[i] > th));
-      for (int bit = 31; bit >= 0; --bit) {
-        const unsigned t = tl | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) n += __popcll(__ballot(hi[i] == th && lo[i] >= t));
-        if (n >= need) tl = t;
-      }
-    }
-    __syncthreads();
-    int at = 0;
-    u64 least = ~0ull;
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const bool keep = hi[i] > th || (hi[i] == th && lo[i] >= tl);
-      const bool real = i * 64 + lane < cnt;
-      const u64 mask = __ballot(keep);
-      if (keep) {
-        const u64 v = ((u64)hi[i] << 32) | lo[i];
-        buf[at + lanes_below(mask)] = v;
-        least = v < least ? v : least;
-      } else if (real) {
-        others.add1(order_value(hi[i]), c);
-      }
-      at += __popcll(mask);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const u64 v = __shfl_xor(least, o, 64);
-      least = v < least ? v : least;
-    }
-    cnt = k;
-    tkey = least;
-    const float t = order_value((unsigned)(least >> 32));
-    tval = t != t ? INFINITY : t;
-    __syncthreads();
-  }
-  // lanes with `has` offer a key; returns true where it was taken (what is not taken belongs to the others)
-  __device__ __forceinline__ bool offer(u64 key, bool has) {
-    bool in = has && key > tkey;
-    u64 mask = __ballot(in);
-    if (!mask) return false;
-    if (cnt + __popcll(mask) > CAP) {
-      cut();
-      in = in && key > tkey;
-      mask = __ballot(in);
-    }
-    if (in) buf[cnt + lanes_below(mask)] = key;
-    cnt += __popcll(mask);
-    return in;
-  }
-  // sort what is left (<= k keys): every key's rank is the number of larger ones
-  template <typename F> __device__ __forceinline__ void finish(F&& emit) {
-    if (cnt > k) cut();
-    __syncthreads();
-    u64 mine[KB / 64];
-    int rank[KB / 64];
-#pragma unroll
-    for (int i = 0; i < KB / 64; ++i) { mine[i] = i * 64 + lane < cnt ? buf[i * 64 + lane] : 0; rank[i] = 0; }
-    for (int j = 0; j < cnt; ++j) {
-      const u64 v = buf[j];
-#pragma unroll
-      for (int i = 0; i < KB / 64; ++i) rank[i] += v > mine[i] ? 1 : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < KB / 64; ++i) if (i * 64 + lane < cnt) emit(rank[i], mine[i]);
-    others.wave(c);
-  }
-};
-
-template <typename E> __device__ __forceinline__ void emit_row(const TopArgs& a, long n, int rank, u64 key) {
-  const float v = order_value((unsigned)(key >> 32));
-  Elt<E>::st(static_cast<E*>(a.values) + n * a.k + rank, v);
-  a.ids[n * a.k + rank] = (long long)(~(unsigned)key);
+// maximum over the wave by data-parallel moves (row shifts of 1, 2, 4, 8, then two broadcasts: lane 63 holds the result)
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#define VLN_DPP_MAX(ctrl) { const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false); v = o > v ? o : v; }
+  VLN_DPP_MAX(0x111) VLN_DPP_MAX(0x112) VLN_DPP_MAX(0x114) VLN_DPP_MAX(0x118) VLN_DPP_MAX(0x142) VLN_DPP_MAX(0x143)
+#undef VLN_DPP_MAX
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ float log_mass(const OnlineSum& o, float invT) {
-  return o.s == 0.f ? -INFINITY : (o.m == INFINITY ? INFINITY : o.m * invT + logf(o.s));
+__device__ __forceinline__ unsigned wave_umin(unsigned v) { return ~wave_umax(~v); }
+
+// The largest t in [lo, hi] that at least `want` of the wave's values reach -- lo must be reached by that many; ends early at a t that
+// exactly `want` reach (`exact`).  count(t): how many values are >= t.
+template <typename F> __device__ __forceinline__ unsigned bisect(unsigned lo, unsigned hi, int want, bool& exact, F&& count) {
+  int n = count(hi);
+  exact = n == want;
+  if (n >= want) return hi;
+  while (hi - lo > 1) {                  // count(lo) >= want > count(hi)
+    const unsigned mid = lo + ((hi - lo) >> 1);
+    n = count(mid);
+    if (n >= want) { lo = mid; if (n == want) { exact = true; return lo; } }
+    else hi = mid;
+  }
+  return lo;
 }
 
-template <typename E, int KB> __global__ __launch_bounds__(64) void top_scan_kernel(TopArgs a) {
-  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC, G = KB / 64;      // G maxima per lane for the first threshold
-  __shared__ u64 buf[Candidates<KB>::CAP];
+template <typename E> __device__ __forceinline__ void emit_row(const TopArgs& a, long n, int rank, unsigned order, unsigned idx) {
+  Elt<E>::st(static_cast<E*>(a.values) + n * a.k + rank, order_value(order));
+  a.ids[n * a.k + rank] = (long long)idx;
+}
+__device__ __forceinline__ float log_mass(float m, float s, float invT) {
+  return s == 0.f ? -INFINITY : (m == INFINITY ? INFINITY : m * invT + logf(s));
+}
+
+// workgroups per CU that the registers are limited to: 4 waves per SIMD hold 64 KB rows, 8 the smaller ones
+template <int W, int NVR> constexpr int row_groups() { return (NVR == 16 ? 4 : NVR == 8 ? 6 : 8) * 4 / W; }
+
+template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W, (row_groups<W, NVR>())) void top_row_kernel(TopArgs a) {
+  constexpr int VEC = RowGeo<E>::VEC, T = 64 * W, CAP = W == 1 ? 256 : 1024, GU = NVR / G;
+  __shared__ u64 cand[CAP];
+  __shared__ unsigned gmax[T * G];
+  __shared__ int count, part[2][W];
+  __shared__ float bound;
+  __shared__ float2 sums[W];
   const long n = blockIdx.x;
-  const int s = blockIdx.y, lane = threadIdx.x;
+  const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   const RowGeo<E> g(p, a.V);
-  Candidates<KB> cd;
-  cd.init(buf, a.k, a.c, lane);
-  const int segv = a.seg / VEC, v0 = min(g.nv, s * segv), v1 = s == a.S - 1 ? g.nv : min(g.nv, v0 + segv);
-  auto single = [&](int col, bool has) {
-    const float x = has ? Elt<E>::ld(p + col) : -INFINITY;
-    const bool in = cd.offer(make_key(x, (unsigned)col), has);
-    if (has && !in) cd.others.add1(x, a.c);
-  };
-  if (s == 0 && g.head) single(lane, lane < g.head);
-  uint4 raw[U];
-  auto fetch = [&](int v) {
+  const int v0 = min(g.nv, s * T * NVR), v1 = min(g.nv, v0 + T * NVR);
+  uint4 raw[NVR];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = v + u * 64 + lane;
-      raw[u] = ld_vec<E>(p + g.head + (int64_t)(i < v1 ? i : v1 - 1) * VEC);
-    }
-  };
-  if (v0 < v1) fetch(v0);
-  for (int v = v0; v < v1; v += 64 * U) {
-    float x[16];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      unpack16<E>(raw[u], x + u * VEC);
-      if (v + u * 64 + lane >= v1) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) x[u * VEC + j] = -INFINITY;
-      }
-    }
-    if (v + 64 * U < v1) fetch(v + 64 * U);
-    float mx = x[0];
-#pragma unroll
-    for (int j = 1; j < 16; ++j) mx = nan_max(mx, x[j]);
-    if (__any(!(mx <= cd.tval))) {
-      if (v == v0) {
-        // the k-th largest of 64 G group maxima (groups beyond the row's end do not count) is reached by at least k elements
-        unsigned gm[G];
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          float m = x[i * (16 / G)];
-#pragma unroll
-          for (int j = 1; j < 16 / G; ++j) m = nan_max(m, x[i * (16 / G) + j]);
-          const int u = i * (16 / G) / VEC;
-          gm[i] = v + u * 64 + lane < v1 ? order_bits(m) : 0u;
-        }
-        unsigned th = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-          const unsigned t = th | (1u << bit);
-          int c = 0;
-#pragma unroll
-          for (int i = 0; i < G; ++i) c += __popcll(__ballot(gm[i] >= t));
-          if (c >= a.k) { th = t; if (c == a.k) break; }
-        }
-        if (th) {
-          const u64 t = ((u64)th << 32) - 1;
-          if (t > cd.tkey) {
-            cd.tkey = t;
-            cd.tval = order_value(th == 0x80000000u ? th - 2 : th - 1);      // below +0 comes -0, which compares equal to it
-          }
-        }
-      }
-      // (the bound of the chunk's start: a cut in between raises tval to a value that elements of THIS chunk may share at a lower index)
-      const float tval = cd.tval;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = v + u * 64 + lane;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const bool may = !(x[u * VEC + j] <= tval);
-          if (__any(may)) {
-            const bool in = cd.offer(make_key(x[u * VEC + j], (unsigned)(g.head + i * VEC + j)), may && i < v1);
-            if (in) x[u * VEC + j] = -INFINITY;
-          }
-        }
-      }
-      // the exact border of what has been seen: later elements equal to it have higher indices and lose
-      if (cd.cnt > cd.k && (v == v0 || cd.cnt > cd.k + KB / 2)) cd.cut();
-      mx = x[0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, x[j]);
-    }
-    cd.others.add_max(x, mx, a.c);
+  for (int u = 0; u < NVR; ++u) {
+    raw[u] = make_uint4(0, 0, 0, 0);
+    if (v0 + u * T + tid < v1) raw[u] = ld_vec<E>(p + g.head + (int64_t)(v0 + u * T + tid) * VEC);
   }
-  if (s == a.S - 1 && g.tail) single(g.tail0() + lane, lane < g.tail);
-  if (a.S == 1) {
-    cd.finish([&](int rank, u64 key) { emit_row<E>(a, n, rank, key); });
-    if (lane == 0) a.rest[n] = log_mass(cd.others, a.invT);
-  } else {
-    u64* o = a.keys + (n * a.S + s) * a.k;
-    cd.finish([&](int rank, u64 key) { o[rank] = key; });
-    for (int i = cd.cnt + lane; i < a.k; i += 64) o[i] = 0;
-    if (lane == 0) a.sums[n * a.S + s] = make_float2(cd.others.m, cd.others.s);
+  // the single elements in front of the first and behind the last vector: threads of the first segment
+  int scol = -1;
+  if (s == 0) scol = tid < g.head ? tid : (tid >= VEC && tid - VEC < g.tail ? g.tail0() + tid - VEC : -1);
+  const float sx = scol >= 0 ? Elt<E>::ld(p + scol) : -INFINITY;
+  if (tid == 0) count = 0;
+#pragma unroll
+  for (int q = 0; q < G; ++q) {
+    float m = -INFINITY;
+    bool has = false;
+#pragma unroll
+    for (int u = q * GU; u < (q + 1) * GU; ++u) {
+      asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w));
+      float x[VEC];
+      unpack16<E>(raw[u], x);
+      float t = x[0];
+#pragma unroll
+      for (int j = 1; j < VEC; ++j) t = nan_max(t, x[j]);
+      if (v0 + u * T + tid < v1) { m = nan_max(m, t); has = true; }
+    }
+    if (q == 0 && scol >= 0) { m = nan_max(m, sx); has = true; }
+    gmax[q * T + tid] = has ? order_bits(m) : 0u;
+  }
+  __syncthreads();
+  if (w == 0) {
+    unsigned gm[W * G], least = 0xffffffffu, most = 0u;
+    int groups = 0;
+#pragma unroll
+    for (int i = 0; i < W * G; ++i) {
+      gm[i] = gmax[i * 64 + lane];
+      groups += __popcll(__ballot(gm[i] != 0u));
+      most = max(most, gm[i]);
+      least = min(least, gm[i] - 1u);          // (0 - 1: an empty group)
+    }
+    float t = __builtin_nanf("");              // fewer groups than k: every element is a candidate
+    if (groups >= a.k) {
+      bool exact;
+      const unsigned th = bisect(wave_umin(least) + 1u, wave_umax(most), a.k, exact, [&](unsigned b) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < W * G; ++i) c += __popcll(__ballot(gm[i] >= b));
+        return c;
+      });
+      t = order_value(th == 0x80000000u ? th - 2 : th - 1);      // just below th (below +0 comes -0, which compares equal to it)
+    }
+    if (lane == 0) bound = t;
+  }
+  __syncthreads();
+  const float tval = bound;
+  OnlineSum others;
+  bool exact = false;                          // only elements of order bits > th, or == th and complemented index >= tl, are candidates
+  unsigned th = 0u, tl = 0u;
+  while (true) {
+    auto offer = [&](float x, int col) {       // false: one of the others
+      const unsigned o = order_bits(x);
+      if (exact && !(o > th || (o == th && ~(unsigned)col >= tl))) return false;
+      const int at = atomicAdd(&count, 1);
+      if (at < CAP) cand[at] = ((u64)o << 32) | (unsigned)~col;
+      return true;
+    };
+#pragma unroll
+    for (int u = 0; u < NVR; ++u) {
+      int i = v0 + u * T + tid;
+      if (v0 + u * T >= v1) continue;           // uniform
+      // (unpacked again, and columns formed, where they are needed: prepared ahead for all vectors they would take three times the registers)
+      asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w), "+v"(i));
+      float x[VEC];
+      unpack16<E>(raw[u], x);
+      float mx = x[0];
+#pragma unroll
+      for (int j = 1; j < VEC; ++j) mx = nan_max(mx, x[j]);
+      if (i >= v1) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = -INFINITY;
+        mx = -INFINITY;
+      }
+      if (__ballot(!(mx <= tval))) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (!(x[j] <= tval) && i < v1 && offer(x[j], g.head + i * VEC + j)) x[j] = -INFINITY;
+        mx = x[0];
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) mx = fmaxf(mx, x[j]);
+      }
+      others.add_max(x, mx, a.c);
+    }
+    if (scol >= 0 && ((sx <= tval) || !offer(sx, scol))) others.add1(sx, a.c);
+    __syncthreads();
+    if (count <= CAP || exact) break;
+    // More reach the bound than the list holds: the exact border, counting the segment's elements per step (read again, from the caches).
+    int turn = 0;
+    auto block_count = [&](auto&& has) {       // has(order bits, complemented index)
+      int c = 0;
+      for (int i = v0 + tid; i < v1; i += T) {
+        float x[VEC];
+        unpack16<E>(ld_vec<E>(p + g.head + (int64_t)i * VEC), x);
+        for (int j = 0; j < VEC; ++j) c += has(order_bits(x[j]), ~(unsigned)(g.head + i * VEC + j)) ? 1 : 0;
+      }
+      if (scol >= 0) c += has(order_bits(sx), ~(unsigned)scol) ? 1 : 0;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+      if (lane == 0) part[turn][w] = c;
+      __syncthreads();
+      c = 0;
+      for (int i = 0; i < W; ++i) c += part[turn][i];
+      turn ^= 1;
+      return c;
+    };
+    bool enough;
+    th = bisect(1u, 0xffffffffu, a.k, enough, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
+    if (!enough) {
+      const int need = a.k - block_count([&](unsigned h, unsigned) { return h > th; });
+      bool e;
+      tl = bisect(0u, 0xffffffffu, need, e, [&](unsigned t) { return block_count([&](unsigned h, unsigned l) { return h == th && l >= t; }); });
+    }
+    exact = true;
+    __syncthreads();
+    if (tid == 0) count = 0;
+    others = OnlineSum();
+    __syncthreads();
+  }
+  const int nc = count;
+  u64* seg = a.S > 1 ? a.keys + (n * a.S + s) * a.k : nullptr;
+  // every candidate to its place; what the places beyond k add to the others then depends on the values only
+  u64 mine[CAP / T];
+  int rank[CAP / T];
+#pragma unroll
+  for (int i = 0; i < CAP / T; ++i) {
+    if (i * T >= nc) continue;
+    mine[i] = i * T + tid < nc ? cand[i * T + tid] : 0ull;
+    int r = 0;
+    for (int j = 0; j < nc; ++j) r += cand[j] > mine[i] ? 1 : 0;
+    rank[i] = r;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < CAP / T; ++i) if (i * T + tid < nc) cand[rank[i]] = mine[i];
+  __syncthreads();
+  for (int c = tid; c < nc; c += T) {
+    const u64 v = cand[c];
+    if (c >= a.k) others.add1(order_value((unsigned)(v >> 32)), a.c);
+    else if (seg) seg[c] = v;
+    else emit_row<E>(a, n, c, (unsigned)(v >> 32), ~(unsigned)v);
+  }
+  if (seg) for (int c = nc + tid; c < a.k; c += T) seg[c] = 0ull;
+  others.wave(a.c);
+  if (lane == 0) sums[w] = make_float2(others.m, others.s);
+  __syncthreads();
+  if (tid == 0) {
+    OnlineSum o;
+    for (int i = 0; i < W; ++i) o.merge(sums[i].x, sums[i].y, a.c);
+    if (seg) a.sums[n * a.S + s] = make_float2(o.m, o.s);
+    else a.rest[n] = log_mass(o.m, o.s, a.invT);
   }
 }
 
-template <typename E, int KB> __global__ __launch_bounds__(64) void top_merge_kernel(TopArgs a) {
-  __shared__ u64 buf[Candidates<KB>::CAP];
+// One workgroup selects the k best of up to `per` segments' candidates: all of them in registers, the k-th best by bisection over the
+// order bits (then, among equal values, over the indices), counting with one barrier per step.  A row with more segments is merged in
+// levels: blockIdx.y is the group, its result one segment of the next level (last level: the row's result).
+constexpr int kMergeThreads = 512, kMergeRegs = 16, kMergeMax = kMergeThreads * kMergeRegs;
+
+template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge_kernel(TopArgs a, int per, u64* keys_out, float2* sums_out) {
+  constexpr int W = kMergeThreads / 64;
+  __shared__ u64 best[VLN_TOP_LOGITS_MAX];
+  __shared__ int part[2][W];
+  __shared__ unsigned ends[2][W];
+  __shared__ float2 sums[W];
+  __shared__ int taken;
   const long n = blockIdx.x;
-  const int lane = threadIdx.x, total = a.S * a.k;
-  Candidates<KB> cd;
-  cd.init(buf, a.k, a.c, lane);
-  for (int i = lane; i < a.S; i += 64) {
-    const float2 o = a.sums[n * a.S + i];
-    cd.others.merge(o.x, o.y, a.c);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, s0 = blockIdx.y * per, segs = min(per, a.S - s0), total = segs * a.k;
+  const u64* keys = a.keys + (n * a.S + s0) * a.k;
+  OnlineSum others;
+  for (int i = tid; i < segs; i += kMergeThreads) {
+    const float2 o = a.sums[n * a.S + s0 + i];
+    others.merge(o.x, o.y, a.c);
   }
-  const u64* keys = a.keys + n * total;
-  for (int i = 0; i < total; i += 64) {
-    const bool has = i + lane < total;
-    const u64 key = has ? keys[i + lane] : 0;
-    const bool in = cd.offer(key, has && key);
-    if (has && key && !in) cd.others.add1(order_value((unsigned)(key >> 32)), a.c);
+  unsigned hi[kMergeRegs], lo[kMergeRegs], least = 0xffffffffu, most = 0;
+  const int regs = (total + kMergeThreads - 1) / kMergeThreads;
+#pragma unroll
+  for (int i = 0; i < kMergeRegs; ++i) {
+    const int at = i * kMergeThreads + tid;
+    const u64 v = i < regs && at < total ? keys[at] : 0ull;
+    hi[i] = (unsigned)(v >> 32); lo[i] = (unsigned)v;
+    most = max(most, hi[i]);
+    least = min(least, v ? hi[i] : 0xffffffffu);
   }
-  cd.finish([&](int rank, u64 key) { emit_row<E>(a, n, rank, key); });
-  if (lane == 0) a.rest[n] = log_mass(cd.others, a.invT);
+  if (tid == 0) taken = 0;
+  if (tid < a.k) best[tid] = 0ull;
+  least = wave_umin(least); most = wave_umax(most);
+  if (lane == 0) { ends[0][w] = least; ends[1][w] = most; }
+  __syncthreads();
+  for (int i = 0; i < W; ++i) { least = min(least, ends[0][i]); most = max(most, ends[1][i]); }
+  int turn = 0;
+  auto block_count = [&](auto&& has) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kMergeRegs; ++i) if (i < regs) c += __popcll(__ballot(has(hi[i], lo[i])));
+    if (lane == 0) part[turn][w] = c;
+    __syncthreads();
+    c = 0;
+    for (int i = 0; i < W; ++i) c += part[turn][i];
+    turn ^= 1;
+    return c;
+  };
+  bool exact = true;
+  unsigned th = 1u, tl = 0u;                 // (a group with no more than k elements keeps them all)
+  if (block_count([&](unsigned h, unsigned) { return h != 0u; }) > a.k)
+    th = bisect(least, most, a.k, exact, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
+  if (!exact) {
+    const int need = a.k - block_count([&](unsigned h, unsigned) { return h > th; });
+    bool e;
+    tl = bisect(0u, 0xffffffffu, need, e, [&](unsigned t) { return block_count([&](unsigned h, unsigned l) { return h == th && l >= t; }); });
+  }
+#pragma unroll
+  for (int i = 0; i < kMergeRegs; ++i) {
+    if (i >= regs) continue;
+    const bool keep = hi[i] > th || (hi[i] == th && lo[i] >= tl);
+    const u64 mask = __ballot(keep);
+    int base = 0;
+    if (mask && lane == 0) base = atomicAdd(&taken, __popcll(mask));
+    base = __builtin_amdgcn_readfirstlane(base);
+    if (keep) best[base + lanes_below(mask)] = ((u64)hi[i] << 32) | lo[i];
+    else if (hi[i]) others.add1(order_value(hi[i]), a.c);
+  }
+  others.wave(a.c);
+  if (lane == 0) sums[w] = make_float2(others.m, others.s);
+  __syncthreads();
+  const long slot = n * gridDim.y + blockIdx.y;
+  if (tid < a.k) {
+    const u64 mine = best[tid];
+    int rank = 0;
+    for (int j = 0; j < a.k; ++j) rank += best[j] > mine ? 1 : 0;
+    if (keys_out) keys_out[slot * a.k + tid] = mine;
+    else emit_row<E>(a, n, rank, (unsigned)(mine >> 32), ~(unsigned)mine);
+  }
+  if (tid == 0) {
+    OnlineSum o;
+    for (int i = 0; i < W; ++i) o.merge(sums[i].x, sums[i].y, a.c);
+    if (keys_out) sums_out[slot] = make_float2(o.m, o.s);
+    else a.rest[n] = log_mass(o.m, o.s, a.invT);
+  }
 }
 
-// Segments per row: as many waves as keep every SIMD busy (16 per CU), but none shorter than four chunks -- each segment costs a
-// threshold search and k keys of traffic.
-static void top_split(int N, int V, int* S, int* seg) {
+struct TopPlan {
+  int W, NVR, G, S, per;        // waves, vectors per thread, groups per thread, segments, segments of one merge
+  int levels; int count[8];     // segments left after each merge level
+};
+// Short rows (<= 256 vectors) with k <= 64: one wave, no barrier to wait for.  Otherwise four waves and the most vectors per thread (16:
+// 64 KB of a row) that still give every CU two workgroups; more, smaller segments otherwise, at least 4 vectors per thread.
+static TopPlan top_plan(int N, int V, int k, int vec) {
+  TopPlan p{};
+  const long nv = ((long)V + vec - 1) / vec;
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  const int want = (16 * cus + N - 1) / N, most = (V + 4095) / 4096;
-  int n = want < most ? want : most;
-  if (n < 1) n = 1;
-  *seg = ((V + n - 1) / n + 1023) / 1024 * 1024;
-  *S = (V + *seg - 1) / *seg;
+  if (nv <= 256 && k <= 64) { p.W = 1; p.NVR = 4; p.G = k <= 16 ? 1 : 4; }
+  else {
+    p.W = 4; p.NVR = 16; p.G = k <= 64 ? 1 : 4;
+    while (p.NVR > 4 && (nv <= 256L * (p.NVR / 2) || (long)N * ((nv + 256L * p.NVR - 1) / (256L * p.NVR)) < 2L * cus)) p.NVR /= 2;
+  }
+  const long held = 64L * p.W * p.NVR;
+  p.S = (int)((nv + held - 1) / held);
+  p.per = kMergeMax / k;
+  for (int n = p.S; n > 1;) { n = (n + p.per - 1) / p.per; p.count[p.levels++] = n; }
+  return p;
+}
+static int64_t top_ws(const TopPlan& p, int N, int k) {
+  int64_t segs = p.S > 1 ? p.S : 0;
+  for (int i = 0; i + 1 < p.levels; ++i) segs += p.count[i];
+  return segs * N * ((int64_t)k * 8 + 8);
 }
 
-template <typename E, int KB> static int top_launch(const TopArgs& a, hipStream_t st) {
-  VLN_LAUNCH((top_scan_kernel<E, KB>), dim3((unsigned)a.N, (unsigned)a.S), dim3(64), 0, st, a);
-  if (a.S > 1) VLN_LAUNCH((top_merge_kernel<E, KB>), dim3((unsigned)a.N), dim3(64), 0, st, a);
+template <typename E, int W, int NVR> static void top_rows(const TopArgs& a, int G, hipStream_t st) {
+  const dim3 grid((unsigned)a.N, (unsigned)a.S);
+  if (G == 1) VLN_LAUNCH((top_row_kernel<E, W, NVR, 1>), grid, dim3(64 * W), 0, st, a);
+  else VLN_LAUNCH((top_row_kernel<E, W, NVR, 4>), grid, dim3(64 * W), 0, st, a);
+}
+template <typename E> static int top_launch(TopArgs a, const TopPlan& p, char* ws, hipStream_t st) {
+  auto take = [&](int segs) {
+    a.keys = reinterpret_cast<u64*>(ws);
+    a.sums = reinterpret_cast<float2*>(ws + (int64_t)a.N * segs * a.k * 8);
+    ws += (int64_t)a.N * segs * (a.k * 8 + 8);
+  };
+  a.S = p.S;
+  if (a.S > 1) take(a.S);
+  if (p.W == 1) top_rows<E, 1, 4>(a, p.G, st);
+  else if (p.NVR == 4) top_rows<E, 4, 4>(a, p.G, st);
+  else if (p.NVR == 8) top_rows<E, 4, 8>(a, p.G, st);
+  else top_rows<E, 4, 16>(a, p.G, st);
+  for (int i = 0; i < p.levels; ++i) {
+    const TopArgs from = a;
+    const bool last = p.count[i] == 1;
+    if (!last) take(p.count[i]);
+    VLN_LAUNCH((top_merge_kernel<E>), dim3((unsigned)a.N, (unsigned)p.count[i]), dim3(kMergeThreads), 0, st, from, p.per, last ? nullptr : a.keys,
+               last ? nullptr : a.sums);
+    a.S = p.count[i];
+  }
   VLN_CHECK_LAUNCH("top_logits");
   return VLN_OK;
-}
-template <typename E> static int top_dispatch(const TopArgs& a, hipStream_t st) {
-  if (a.k <= 64) return top_launch<E, 64>(a, st);
-  if (a.k <= 128) return top_launch<E, 128>(a, st);
-  return top_launch<E, 256>(a, st);
 }
 
 }  // namespace vln
 
-extern "C" int64_t vln_top_logits_ws_bytes(int N, int V, int k) {
-  if (N <= 0 || V <= 0 || k <= 0) return 0;
-  int S, seg;
-  vln::top_split(N, V, &S, &seg);
-  return S > 1 ? (int64_t)N * S * ((int64_t)k * 8 + 8) : 0;
+extern "C" int64_t vln_top_logits_ws_bytes(int N, int V, int type, int k) {
+  if (N <= 0 || V <= 0 || k <= 0 || k > VLN_TOP_LOGITS_MAX || (type != VLN_F32 && type != VLN_BF16)) return 0;
+  return vln::top_ws(vln::top_plan(N, V, k, type == VLN_F32 ? 4 : 8), N, k);
 }
 extern "C" int vln_top_logits(const void* logits, int64_t ld, int type, int N, int V, int k, float temperature, void* values, int64_t* ids,
                               float* rest, void* ws, int64_t ws_bytes, vln_stream_t s) {
   if (!logits || !values || !ids || !rest || N <= 0 || V <= 0 || ld < V) { vln::set_error("vln_top_logits: bad args"); return VLN_ERR_ARG; }
+  if (type != VLN_F32 && type != VLN_BF16) { vln::set_error("vln_top_logits: type must be fp32 or bf16"); return VLN_ERR_ARG; }
   if (k < 1 || k > V || k > VLN_TOP_LOGITS_MAX) { vln::set_error("vln_top_logits: k must be 1 .. min(V, %d)", VLN_TOP_LOGITS_MAX); return VLN_ERR_ARG; }
   if (!(temperature >= VLN_TEMPERATURE_MIN && temperature <= VLN_TEMPERATURE_MAX)) { vln::set_error("vln_top_logits: bad temperature"); return VLN_ERR_ARG; }
+  const vln::TopPlan p = vln::top_plan(N, V, k, type == VLN_F32 ? 4 : 8);
+  const int64_t need = vln::top_ws(p, N, k);
+  if (need && (!ws || ws_bytes < need)) { vln::set_error("vln_top_logits: workspace too small"); return VLN_ERR_ARG; }
   vln::TopArgs a{};
   a.logits = logits; a.ld = ld; a.N = N; a.V = V; a.k = k;
-  vln::top_split(N, V, &a.S, &a.seg);
-  if (a.S > 1) {
-    if (!ws || ws_bytes < vln_top_logits_ws_bytes(N, V, k)) { vln::set_error("vln_top_logits: workspace too small"); return VLN_ERR_ARG; }
-    a.keys = static_cast<vln::u64*>(ws);
-    a.sums = reinterpret_cast<float2*>(a.keys + (int64_t)N * a.S * k);
-  }
   a.c = vln::kLog2e / temperature; a.invT = 1.f / temperature;
   a.values = values; a.ids = (long long*)ids; a.rest = rest;
-  if (type == VLN_F32) return vln::top_dispatch<float>(a, (hipStream_t)s);
-  if (type == VLN_BF16) return vln::top_dispatch<bf16_raw>(a, (hipStream_t)s);
-  vln::set_error("vln_top_logits: type must be fp32 or bf16");
-  return VLN_ERR_ARG;
+  if (type == VLN_F32) return vln::top_launch<float>(a, p, static_cast<char*>(ws), (hipStream_t)s);
+  return vln::top_launch<bf16_raw>(a, p, static_cast<char*>(ws), (hipStream_t)s);
 }

@@ -250,7 +250,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     if N:
         lib = _lib.load()
         with _on(dev):
-            nb = lib.vln_top_logits_ws_bytes(N, V, k)
+            nb = lib.vln_top_logits_ws_bytes(N, V, _TYPES[z.dtype], k)
             ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
             _lib.check(lib.vln_top_logits(z.data_ptr(), _ld(z), _TYPES[z.dtype], N, V, k, T, values.data_ptr(), ids.data_ptr(), rest.data_ptr(),
                                           _p(ws), nb, _lib.raw_stream()), "vln_top_logits")

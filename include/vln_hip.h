@@ -376,7 +376,7 @@ int vln_constrain_logits(const vln_constrain* args, vln_stream_t s);
 #define VLN_TOP_LOGITS_MAX 256
 #define VLN_TEMPERATURE_MIN 1e-3f
 #define VLN_TEMPERATURE_MAX 1e3f
-int64_t vln_top_logits_ws_bytes(int N, int V, int k);
+int64_t vln_top_logits_ws_bytes(int N, int V, int type, int k);
 int vln_top_logits(const void* logits, int64_t ld, int type, int N, int V, int k, float temperature, void* values, int64_t* ids,
                    float* rest, void* ws, int64_t ws_bytes, vln_stream_t s);
 

@@ -129,7 +129,7 @@ def test_c_abi_refusals(vln):
         assert top(**kw) == 1, kw
         assert b"vln_top_logits" in lib.vln_last_error_string()
     assert top(V=1000, ld=1000, k=257) == 1
-    assert lib.vln_top_logits_ws_bytes(1, 131072, 128) > 0 and lib.vln_top_logits_ws_bytes(0, 10, 1) == 0
+    assert lib.vln_top_logits_ws_bytes(1, 131072, 0, 128) > 0 and lib.vln_top_logits_ws_bytes(0, 10, 0, 1) == 0
 
     def distill(bwd=False, **kw):
         a = L.Distill(p, 40, p, 3, p, 3, None, None, -1, p, p, 1.0, 1.0, 0, 0, 2, 40, 3, 0)
