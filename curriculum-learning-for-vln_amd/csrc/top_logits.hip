@@ -30,23 +30,33 @@ __device__ __forceinline__ float order_value(unsigned o) {
 
 struct TopArgs {
   const void* logits; int64_t ld;
-  int N, V, k, S;                  // S segments per row
+  int N, V, k, S, ks, vps;         // S segments per row of vps vectors, ks candidates of a segment
   float c, invT;                   // log2(e) / T, 1 / T
   void* values; long long* ids; float* rest;
-  u64* keys; float2* sums;         // S > 1: [N, S, k] (order bits << 32 | ~index; 0: none) and [N, S]
+  u64* keys; float2* sums;         // S > 1: [N, S, ks] (order bits << 32 | ~index; 0: none) and [N, S]
 };
 
 __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // NaN wins (v_maximum3_f32)
 
-// maximum over the wave by data-parallel moves (row shifts of 1, 2, 4, 8, then two broadcasts: lane 63 holds the result)
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#define VLN_DPP_MAX(ctrl) { const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false); v = o > v ? o : v; }
-  VLN_DPP_MAX(0x111) VLN_DPP_MAX(0x112) VLN_DPP_MAX(0x114) VLN_DPP_MAX(0x118) VLN_DPP_MAX(0x142) VLN_DPP_MAX(0x143)
-#undef VLN_DPP_MAX
-  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
-}
-__device__ __forceinline__ unsigned wave_umin(unsigned v) { return ~wave_umax(~v); }
-
+// Largest element of a vector, an UNDERESTIMATE where it holds NaN or infinities (enough for a bound that k elements must reach).  bf16: of
+// the pair in a register, the upper element is taken with the lower one as extra mantissa bits -- the order of the upper ones is kept, and
+// cutting the bits off afterwards gives the exact largest -- so only the lower elements are unpacked.
+template <typename E> struct VecMax;
+template <> struct VecMax<float> {
+  float m = -INFINITY;
+  __device__ __forceinline__ void add(const uint4& r) {
+    m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))));
+  }
+  __device__ __forceinline__ float get() const { return m; }
+};
+template <> struct VecMax<bf16_raw> {
+  float lo = -INFINITY, hi = -INFINITY;
+  __device__ __forceinline__ void add(const uint4& r) {
+    hi = fmaxf(hi, fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))));
+    lo = fmaxf(lo, fmaxf(fmaxf(__uint_as_float(r.x << 16), __uint_as_float(r.y << 16)), fmaxf(__uint_as_float(r.z << 16), __uint_as_float(r.w << 16))));
+  }
+  __device__ __forceinline__ float get() const { return fmaxf(lo, __uint_as_float(__float_as_uint(hi) & 0xffff0000u)); }
+};
 // The largest t in [lo, hi] that at least `want` of the wave's values reach -- lo must be reached by that many; ends early at a t that
 // exactly `want` reach (`exact`).  count(t): how many values are >= t.
 template <typename F> __device__ __forceinline__ unsigned bisect(unsigned lo, unsigned hi, int want, bool& exact, F&& count) {
@@ -61,6 +71,44 @@ template <typename F> __device__ __forceinline__ unsigned bisect(unsigned lo, un
   }
   return lo;
 }
+// Some t in [lo, hi] that at least `want` and, if few steps find it, at most `most` values reach: a bound need not be exact.
+template <typename F> __device__ __forceinline__ unsigned bisect_near(unsigned lo, unsigned hi, int want, int most, int steps, F&& count) {
+  if (count(hi) >= want) return hi;
+  while (hi - lo > 1 && steps-- > 0) {
+    const unsigned mid = lo + ((hi - lo) >> 1);
+    const int n = count(mid);
+    if (n >= want) { lo = mid; if (n <= most) break; }
+    else hi = mid;
+  }
+  return lo;
+}
+// Calls emit(place, key) for the nc keys of an LDS list, place = the number of larger ones.  Threads that are left over share the
+// comparisons of a key: T / C threads each look at a part of the list (C: the power of two from 64 that holds nc).  Ends with the places
+// emitted by the threads below nc; every thread of the workgroup calls it.
+template <int T, typename F> __device__ __forceinline__ void place_by_rank(const u64* cand, int* place, int nc, int tid, F&& emit) {
+  int C = 64;
+  while (C < nc && C < T) C *= 2;
+  const int P = T / C, part = tid / C, step = ((nc + P - 1) / P + 1) & ~1;      // an even share each
+  const int j0 = min(nc, part * step), j1 = min(nc, j0 + step);
+  if (P > 1) {
+    if (tid < C) place[tid] = 0;
+    __syncthreads();
+  }
+  for (int c = tid & (C - 1); c < nc; c += C) {
+    const u64 mine = cand[c];
+    const ulonglong2* l = reinterpret_cast<const ulonglong2*>(cand + j0);
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < (j1 - j0) / 2; ++j) { const ulonglong2 q = l[j]; r += (q.x > mine ? 1 : 0) + (q.y > mine ? 1 : 0); }
+    if ((j1 - j0) & 1) r += cand[j1 - 1] > mine ? 1 : 0;
+    if (P > 1) atomicAdd(&place[c], r);
+    else emit(r, mine);
+  }
+  if (P > 1) {
+    __syncthreads();
+    if (tid < nc) emit(place[tid], cand[tid]);
+  }
+}
 
 template <typename E> __device__ __forceinline__ void emit_row(const TopArgs& a, long n, int rank, unsigned order, unsigned idx) {
   Elt<E>::st(static_cast<E*>(a.values) + n * a.k + rank, order_value(order));
@@ -71,47 +119,44 @@ __device__ __forceinline__ float log_mass(float m, float s, float invT) {
 }
 
 // workgroups per CU that the registers are limited to: 4 waves per SIMD hold 64 KB rows, 8 the smaller ones
-template <int W, int NVR> constexpr int row_groups() { return (NVR == 16 ? 4 : NVR == 8 ? 6 : 8) * 4 / W; }
+template <int W, int NVR> constexpr int row_groups() { return (NVR == 16 ? 4 : NVR == 8 ? 6 : 7) * 4 / W; }
 
 template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W, (row_groups<W, NVR>())) void top_row_kernel(TopArgs a) {
-  constexpr int VEC = RowGeo<E>::VEC, T = 64 * W, CAP = W == 1 ? 256 : 1024, GU = NVR / G;
-  __shared__ u64 cand[CAP];
+  constexpr int VEC = RowGeo<E>::VEC, T = 64 * W, CAP = VLN_TOP_LOGITS_MAX, GU = NVR / G;      // CAP: candidates of a wave
+  __shared__ alignas(16) u64 cand[W * CAP];                   // (first: {value bits, column}, a list per wave)
+  __shared__ int place[T];
   __shared__ unsigned gmax[T * G];
-  __shared__ int count, part[2][W];
+  __shared__ int counts[W], redo, part[2][W];
   __shared__ float bound;
   __shared__ float2 sums[W];
   const long n = blockIdx.x;
   const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   const RowGeo<E> g(p, a.V);
-  const int v0 = min(g.nv, s * T * NVR), v1 = min(g.nv, v0 + T * NVR);
+  const int v0 = min(g.nv, s * a.vps), v1 = min(g.nv, v0 + a.vps);
   uint4 raw[NVR];
 #pragma unroll
   for (int u = 0; u < NVR; ++u) {
-    raw[u] = make_uint4(0, 0, 0, 0);
+    constexpr unsigned none = sizeof(E) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf elements
+    raw[u] = make_uint4(none, none, none, none);
     if (v0 + u * T + tid < v1) raw[u] = ld_vec<E>(p + g.head + (int64_t)(v0 + u * T + tid) * VEC);
   }
   // the single elements in front of the first and behind the last vector: threads of the first segment
   int scol = -1;
   if (s == 0) scol = tid < g.head ? tid : (tid >= VEC && tid - VEC < g.tail ? g.tail0() + tid - VEC : -1);
   const float sx = scol >= 0 ? Elt<E>::ld(p + scol) : -INFINITY;
-  if (tid == 0) count = 0;
+  if (tid == 0) redo = 0;
+  float tmax = sx;
 #pragma unroll
   for (int q = 0; q < G; ++q) {
-    float m = -INFINITY;
-    bool has = false;
+    VecMax<E> m;
 #pragma unroll
-    for (int u = q * GU; u < (q + 1) * GU; ++u) {
-      asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w));
-      float x[VEC];
-      unpack16<E>(raw[u], x);
-      float t = x[0];
-#pragma unroll
-      for (int j = 1; j < VEC; ++j) t = nan_max(t, x[j]);
-      if (v0 + u * T + tid < v1) { m = nan_max(m, t); has = true; }
-    }
-    if (q == 0 && scol >= 0) { m = nan_max(m, sx); has = true; }
-    gmax[q * T + tid] = has ? order_bits(m) : 0u;
+    for (int u = q * GU; u < (q + 1) * GU; ++u) m.add(raw[u]);
+    float t = m.get();
+    bool has = v0 + q * GU * T + tid < v1;
+    if (q == 0 && scol >= 0) { t = fmaxf(t, sx); has = true; }
+    tmax = fmaxf(tmax, t);
+    gmax[q * T + tid] = has ? order_bits(t) : 0u;
   }
   __syncthreads();
   if (w == 0) {
@@ -126,12 +171,11 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
     }
     float t = __builtin_nanf("");              // fewer groups than k: every element is a candidate
     if (groups >= a.k) {
-      bool exact;
-      const unsigned th = bisect(wave_umin(least) + 1u, wave_umax(most), a.k, exact, [&](unsigned b) {
+      const unsigned th = bisect_near(wave_umin(least) + 1u, wave_umax(most), a.k, a.k + a.k / 8 + 2, 12, [&](unsigned b) {
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < W * G; ++i) c += __popcll(__ballot(gm[i] >= b));
-        return c;
+        for (int i = 0; i < W * G; ++i) c += gm[i] >= b ? 1 : 0;
+        return wave_isum(c);
       });
       t = order_value(th == 0x80000000u ? th - 2 : th - 1);      // just below th (below +0 comes -0, which compares equal to it)
     }
@@ -139,46 +183,96 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   }
   __syncthreads();
   const float tval = bound;
+  // The others' sum.  Every element that is no candidate is at most ref = min(the thread's largest, the bound), so the exponentials are
+  // taken relative to ref, one fused multiply-add each (the rounding of ref * c is taken out again at the end).  Where that is no good
+  // reference -- not finite, or everything below it underflows -- the sweep is repeated with a running maximum (`slow`).
   OnlineSum others;
+  float ref = fminf(tmax, tval);
+  bool slow = __ballot(!(fabsf(ref) < 1e30f) && ref != -INFINITY) != 0;
+  if (!(fabsf(ref) < 1e30f)) ref = 0.f;
+  const float nm = -ref * a.c, cut_off = fmaf(ref, a.c, nm);
+  bool redone = false;
   bool exact = false;                          // only elements of order bits > th, or == th and complemented index >= tl, are candidates
   unsigned th = 0u, tl = 0u;
+  constexpr int UV = 8 / VEC;                  // vectors of 8 elements
   while (true) {
-    auto offer = [&](float x, int col) {       // false: one of the others
+    int len = 0;                               // this wave's list
+    uint2* list = reinterpret_cast<uint2*>(cand) + w * CAP;
+    auto wanted = [&](float x, int col) {      // of an element above the bound
+      if (!exact) return true;
       const unsigned o = order_bits(x);
-      if (exact && !(o > th || (o == th && ~(unsigned)col >= tl))) return false;
-      const int at = atomicAdd(&count, 1);
-      if (at < CAP) cand[at] = ((u64)o << 32) | (unsigned)~col;
-      return true;
+      return o > th || (o == th && ~(unsigned)col >= tl);
     };
+    float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < NVR; ++u) {
+    for (int u = 0; u < NVR; u += UV) {
       int i = v0 + u * T + tid;
       if (v0 + u * T >= v1) continue;           // uniform
-      // (unpacked again, and columns formed, where they are needed: prepared ahead for all vectors they would take three times the registers)
-      asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w), "+v"(i));
-      float x[VEC];
-      unpack16<E>(raw[u], x);
+      // (unpacked, and columns formed, where they are needed: prepared ahead for all vectors they would take three times the registers)
+#pragma unroll
+      for (int h = 0; h < UV; ++h) asm volatile("" : "+v"(raw[u + h].x), "+v"(raw[u + h].y), "+v"(raw[u + h].z), "+v"(raw[u + h].w), "+v"(i));
+      float x[8];
+#pragma unroll
+      for (int h = 0; h < UV; ++h) unpack16<E>(raw[u + h], x + h * VEC);
       float mx = x[0];
 #pragma unroll
-      for (int j = 1; j < VEC; ++j) mx = nan_max(mx, x[j]);
-      if (i >= v1) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) x[j] = -INFINITY;
-        mx = -INFINITY;
-      }
+      for (int j = 1; j < 8; ++j) mx = nan_max(mx, x[j]);
       if (__ballot(!(mx <= tval))) {
+int mine = 0, total;
+        bool in[8];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (!(x[j] <= tval) && i < v1 && offer(x[j], g.head + i * VEC + j)) x[j] = -INFINITY;
-        mx = x[0];
+        for (int j = 0; j < 8; ++j) {
+          const int iv = i + j / VEC * T;
+          in[j] = !(x[j] <= tval) && iv < v1 && wanted(x[j], g.head + iv * VEC + j % VEC);
+          mine += in[j] ? 1 : 0;
+        }
+        int at = len - mine + wave_scan(mine, total);
+        len += total;
 #pragma unroll
-        for (int j = 1; j < VEC; ++j) mx = fmaxf(mx, x[j]);
+        for (int j = 0; j < 8; ++j) {
+          if (in[j]) {
+            if (at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), g.head + (i + j / VEC * T) * VEC + j % VEC);
+            ++at;
+            x[j] = -INFINITY;
+          }
+        }
       }
-      others.add_max(x, mx, a.c);
+      if (!slow) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += exp2_hw(fmaf(x[j], a.c, nm));
+      } else {
+        others.add(x, a.c);
+      }
     }
-    if (scol >= 0 && ((sx <= tval) || !offer(sx, scol))) others.add1(sx, a.c);
+    if (!slow) {
+      if (sum != 0.f) { others.m = ref; others.s = sum * exp2_hw(-cut_off); }
+      if (sum < 1e-30f) {                       // masked words only, or an underflow?
+        for (int u = v0 + tid; u < v1; u += T) {
+          float x[VEC];
+          unpack16<E>(ld_vec<E>(p + g.head + (int64_t)u * VEC), x);
+          for (int j = 0; j < VEC; ++j) if (x[j] <= tval && x[j] != -INFINITY) redo = 1;
+        }
+      }
+    }
+    if (s == 0) {
+      const bool in = scol >= 0 && !(sx <= tval) && wanted(sx, scol);
+      int total;
+      const int at = len - 1 + wave_scan(in ? 1 : 0, total);
+      len += total;
+      if (in) { if (at < CAP) list[at] = make_uint2(__float_as_uint(sx), scol); }
+      else if (scol >= 0) others.add1(sx, a.c);
+    }
+    if (lane == 0) counts[w] = len;
     __syncthreads();
-    if (count <= CAP || exact) break;
+    bool full = false;
+#pragma unroll
+    for (int i = 0; i < W; ++i) full = full || counts[i] > CAP;
+    const bool again = redo != 0 && !redone;   // (the same in every wave; `slow` may differ)
+    if (!full && !again) break;
+    if (again) slow = redone = true;
+    others = OnlineSum();
+    __syncthreads();
+    if (!full) continue;
     // More reach the bound than the list holds: the exact border, counting the segment's elements per step (read again, from the caches).
     int turn = 0;
     auto block_count = [&](auto&& has) {       // has(order bits, complemented index)
@@ -205,36 +299,30 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
       bool e;
       tl = bisect(0u, 0xffffffffu, need, e, [&](unsigned t) { return block_count([&](unsigned h, unsigned l) { return h == th && l >= t; }); });
     }
-    exact = true;
-    __syncthreads();
-    if (tid == 0) count = 0;
-    others = OnlineSum();
-    __syncthreads();
+    exact = slow = redone = true;              // (others may now lie above the bound)
   }
-  const int nc = count;
-  u64* seg = a.S > 1 ? a.keys + (n * a.S + s) * a.k : nullptr;
-  // every candidate to its place; what the places beyond k add to the others then depends on the values only
-  u64 mine[CAP / T];
-  int rank[CAP / T];
+  // the waves' lists as one list of keys, in a fixed order
+  int nc = 0, before = 0;
 #pragma unroll
-  for (int i = 0; i < CAP / T; ++i) {
-    if (i * T >= nc) continue;
-    mine[i] = i * T + tid < nc ? cand[i * T + tid] : 0ull;
-    int r = 0;
-    for (int j = 0; j < nc; ++j) r += cand[j] > mine[i] ? 1 : 0;
-    rank[i] = r;
-  }
+  for (int i = 0; i < W; ++i) { if (i == w) before = nc; nc += counts[i]; }
+  uint2 e[CAP / 64];
+#pragma unroll
+  for (int i = 0; i < CAP / 64; ++i) if (i * 64 + lane < counts[w]) e[i] = reinterpret_cast<const uint2*>(cand)[w * CAP + i * 64 + lane];
+  u64* seg = a.S > 1 ? a.keys + (n * a.S + s) * a.ks : nullptr;
+  u64* to = seg && nc <= a.ks ? seg + before : cand + before;      // a segment's candidates need no order
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < CAP / T; ++i) if (i * T + tid < nc) cand[rank[i]] = mine[i];
-  __syncthreads();
-  for (int c = tid; c < nc; c += T) {
-    const u64 v = cand[c];
-    if (c >= a.k) others.add1(order_value((unsigned)(v >> 32)), a.c);
-    else if (seg) seg[c] = v;
-    else emit_row<E>(a, n, c, (unsigned)(v >> 32), ~(unsigned)v);
+  for (int i = 0; i < CAP / 64; ++i)
+    if (i * 64 + lane < counts[w]) to[i * 64 + lane] = ((u64)order_bits(__uint_as_float(e[i].x)) << 32) | ~e[i].y;
+  if (seg) for (int c = min(nc, a.ks) + tid; c < a.ks; c += T) seg[c] = 0ull;
+  if (!seg || nc > a.ks) {
+    __syncthreads();
+    place_by_rank<T>(cand, place, nc, tid, [&](int at, u64 v) {
+      if (at >= (seg ? a.ks : a.k)) others.add1(order_value((unsigned)(v >> 32)), a.c);
+      else if (seg) seg[at] = v;
+      else emit_row<E>(a, n, at, (unsigned)(v >> 32), ~(unsigned)v);
+    });
   }
-  if (seg) for (int c = nc + tid; c < a.k; c += T) seg[c] = 0ull;
   others.wave(a.c);
   if (lane == 0) sums[w] = make_float2(others.m, others.s);
   __syncthreads();
@@ -246,21 +334,22 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   }
 }
 
-// One workgroup selects the k best of up to `per` segments' candidates: all of them in registers, the k-th best by bisection over the
-// order bits (then, among equal values, over the indices), counting with one barrier per step.  A row with more segments is merged in
-// levels: blockIdx.y is the group, its result one segment of the next level (last level: the row's result).
-constexpr int kMergeThreads = 512, kMergeRegs = 16, kMergeMax = kMergeThreads * kMergeRegs;
+// One workgroup selects the k best of up to `per` segments' candidates, all of them in registers: a bound that at least k reach by
+// bisection over the order bits (one barrier per step), which stops as soon as no more than kMergeList do; these are then placed by rank.
+// Only where that many are equal is the border searched among the indices too.  A row with more segments is merged in levels: blockIdx.y
+// is the group, its result one segment of the next level (last level: the row's result).
+constexpr int kMergeThreads = 512, kMergeRegs = 16, kMergeMax = kMergeThreads * kMergeRegs, kMergeList = 512;
 
 template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge_kernel(TopArgs a, int per, u64* keys_out, float2* sums_out) {
   constexpr int W = kMergeThreads / 64;
-  __shared__ u64 best[VLN_TOP_LOGITS_MAX];
+  __shared__ alignas(16) u64 cand[kMergeList];
+  __shared__ int place[kMergeThreads];
   __shared__ int part[2][W];
   __shared__ unsigned ends[2][W];
   __shared__ float2 sums[W];
-  __shared__ int taken;
   const long n = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, s0 = blockIdx.y * per, segs = min(per, a.S - s0), total = segs * a.k;
-  const u64* keys = a.keys + (n * a.S + s0) * a.k;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, s0 = blockIdx.y * per, segs = min(per, a.S - s0), total = segs * a.ks;
+  const u64* keys = a.keys + (n * a.S + s0) * a.ks;
   OnlineSum others;
   for (int i = tid; i < segs; i += kMergeThreads) {
     const float2 o = a.sums[n * a.S + s0 + i];
@@ -276,55 +365,59 @@ template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge
     most = max(most, hi[i]);
     least = min(least, v ? hi[i] : 0xffffffffu);
   }
-  if (tid == 0) taken = 0;
-  if (tid < a.k) best[tid] = 0ull;
   least = wave_umin(least); most = wave_umax(most);
   if (lane == 0) { ends[0][w] = least; ends[1][w] = most; }
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < W; ++i) { least = min(least, ends[0][i]); most = max(most, ends[1][i]); }
-  int turn = 0;
+  int turn = 0, before;                       // before: what the waves in front of this one counted
   auto block_count = [&](auto&& has) {
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < kMergeRegs; ++i) if (i < regs) c += __popcll(__ballot(has(hi[i], lo[i])));
+    for (int i = 0; i < kMergeRegs; ++i) if (i < regs) c += has(hi[i], lo[i]) ? 1 : 0;
+    c = wave_isum(c);
     if (lane == 0) part[turn][w] = c;
     __syncthreads();
-    c = 0;
-    for (int i = 0; i < W; ++i) c += part[turn][i];
+    c = before = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) { if (i == w) before = c; c += part[turn][i]; }
     turn ^= 1;
     return c;
   };
-  bool exact = true;
-  unsigned th = 1u, tl = 0u;                 // (a group with no more than k elements keeps them all)
-  if (block_count([&](unsigned h, unsigned) { return h != 0u; }) > a.k)
-    th = bisect(least, most, a.k, exact, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
-  if (!exact) {
-    const int need = a.k - block_count([&](unsigned h, unsigned) { return h > th; });
-    bool e;
-    tl = bisect(0u, 0xffffffffu, need, e, [&](unsigned t) { return block_count([&](unsigned h, unsigned l) { return h == th && l >= t; }); });
+  unsigned th = 1u, tl = 0u;
+  int nc = block_count([&](unsigned h, unsigned) { return h != 0u; });
+  const int near = min(a.k + a.k / 4 + 32, kMergeList);
+  if (nc > near) {
+    th = bisect_near(least, most, a.k, near, 32, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
+    nc = block_count([&](unsigned h, unsigned) { return h >= th; });
+    if (nc > kMergeList) {
+      const int need = a.k - block_count([&](unsigned h, unsigned) { return h > th; });
+      bool e;
+      tl = bisect(0u, 0xffffffffu, need, e, [&](unsigned t) { return block_count([&](unsigned h, unsigned l) { return h == th && l >= t; }); });
+      nc = block_count([&](unsigned h, unsigned l) { return h > th || (h == th && l >= tl); });
+    }
   }
+  int mine = 0, all;
+#pragma unroll
+  for (int i = 0; i < kMergeRegs; ++i) if (i < regs) mine += hi[i] > th || (hi[i] == th && lo[i] >= tl) ? 1 : 0;
+  int at = before - mine + wave_scan(mine, all);
 #pragma unroll
   for (int i = 0; i < kMergeRegs; ++i) {
     if (i >= regs) continue;
-    const bool keep = hi[i] > th || (hi[i] == th && lo[i] >= tl);
-    const u64 mask = __ballot(keep);
-    int base = 0;
-    if (mask && lane == 0) base = atomicAdd(&taken, __popcll(mask));
-    base = __builtin_amdgcn_readfirstlane(base);
-    if (keep) best[base + lanes_below(mask)] = ((u64)hi[i] << 32) | lo[i];
+    if (hi[i] > th || (hi[i] == th && lo[i] >= tl)) cand[at++] = ((u64)hi[i] << 32) | lo[i];
     else if (hi[i]) others.add1(order_value(hi[i]), a.c);
   }
+  __syncthreads();
+  const long slot = n * gridDim.y + blockIdx.y;
+  if (keys_out) for (int c = min(nc, a.k) + tid; c < a.ks; c += kMergeThreads) keys_out[slot * a.ks + c] = 0ull;
+  place_by_rank<kMergeThreads>(cand, place, nc, tid, [&](int at, u64 v) {
+    if (at >= a.k) others.add1(order_value((unsigned)(v >> 32)), a.c);
+    else if (keys_out) keys_out[slot * a.ks + at] = v;
+    else emit_row<E>(a, n, at, (unsigned)(v >> 32), ~(unsigned)v);
+  });
   others.wave(a.c);
   if (lane == 0) sums[w] = make_float2(others.m, others.s);
   __syncthreads();
-  const long slot = n * gridDim.y + blockIdx.y;
-  if (tid < a.k) {
-    const u64 mine = best[tid];
-    int rank = 0;
-    for (int j = 0; j < a.k; ++j) rank += best[j] > mine ? 1 : 0;
-    if (keys_out) keys_out[slot * a.k + tid] = mine;
-    else emit_row<E>(a, n, rank, (unsigned)(mine >> 32), ~(unsigned)mine);
-  }
   if (tid == 0) {
     OnlineSum o;
     for (int i = 0; i < W; ++i) o.merge(sums[i].x, sums[i].y, a.c);
@@ -334,7 +427,7 @@ template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge
 }
 
 struct TopPlan {
-  int W, NVR, G, S, per;        // waves, vectors per thread, groups per thread, segments, segments of one merge
+  int W, NVR, G, S, vps, ks, per;       // waves, vectors per thread, groups per thread; segments, vectors and candidates of one, segments of one merge
   int levels; int count[8];     // segments left after each merge level
 };
 // Short rows (<= 256 vectors) with k <= 64: one wave, no barrier to wait for.  Otherwise four waves and the most vectors per thread (16:
@@ -350,14 +443,16 @@ static TopPlan top_plan(int N, int V, int k, int vec) {
   }
   const long held = 64L * p.W * p.NVR;
   p.S = (int)((nv + held - 1) / held);
-  p.per = kMergeMax / k;
+  p.vps = (int)((nv + p.S - 1) / p.S);      // equal ones: a short last segment would have too few maxima for a bound
+  p.ks = k + k / 2 + 32;        // (k and the few more that reach a bound)
+  p.per = kMergeMax / p.ks;
   for (int n = p.S; n > 1;) { n = (n + p.per - 1) / p.per; p.count[p.levels++] = n; }
   return p;
 }
-static int64_t top_ws(const TopPlan& p, int N, int k) {
+static int64_t top_ws(const TopPlan& p, int N) {
   int64_t segs = p.S > 1 ? p.S : 0;
   for (int i = 0; i + 1 < p.levels; ++i) segs += p.count[i];
-  return segs * N * ((int64_t)k * 8 + 8);
+  return segs * N * ((int64_t)p.ks * 8 + 8);
 }
 
 template <typename E, int W, int NVR> static void top_rows(const TopArgs& a, int G, hipStream_t st) {
@@ -368,10 +463,10 @@ template <typename E, int W, int NVR> static void top_rows(const TopArgs& a, int
 template <typename E> static int top_launch(TopArgs a, const TopPlan& p, char* ws, hipStream_t st) {
   auto take = [&](int segs) {
     a.keys = reinterpret_cast<u64*>(ws);
-    a.sums = reinterpret_cast<float2*>(ws + (int64_t)a.N * segs * a.k * 8);
-    ws += (int64_t)a.N * segs * (a.k * 8 + 8);
+    a.sums = reinterpret_cast<float2*>(ws + (int64_t)a.N * segs * a.ks * 8);
+    ws += (int64_t)a.N * segs * (a.ks * 8 + 8);
   };
-  a.S = p.S;
+  a.S = p.S; a.ks = p.ks; a.vps = p.vps;
   if (a.S > 1) take(a.S);
   if (p.W == 1) top_rows<E, 1, 4>(a, p.G, st);
   else if (p.NVR == 4) top_rows<E, 4, 4>(a, p.G, st);
@@ -393,7 +488,7 @@ template <typename E> static int top_launch(TopArgs a, const TopPlan& p, char* w
 
 extern "C" int64_t vln_top_logits_ws_bytes(int N, int V, int type, int k) {
   if (N <= 0 || V <= 0 || k <= 0 || k > VLN_TOP_LOGITS_MAX || (type != VLN_F32 && type != VLN_BF16)) return 0;
-  return vln::top_ws(vln::top_plan(N, V, k, type == VLN_F32 ? 4 : 8), N, k);
+  return vln::top_ws(vln::top_plan(N, V, k, type == VLN_F32 ? 4 : 8), N);
 }
 extern "C" int vln_top_logits(const void* logits, int64_t ld, int type, int N, int V, int k, float temperature, void* values, int64_t* ids,
                               float* rest, void* ws, int64_t ws_bytes, vln_stream_t s) {
@@ -402,7 +497,7 @@ extern "C" int vln_top_logits(const void* logits, int64_t ld, int type, int N, i
   if (k < 1 || k > V || k > VLN_TOP_LOGITS_MAX) { vln::set_error("vln_top_logits: k must be 1 .. min(V, %d)", VLN_TOP_LOGITS_MAX); return VLN_ERR_ARG; }
   if (!(temperature >= VLN_TEMPERATURE_MIN && temperature <= VLN_TEMPERATURE_MAX)) { vln::set_error("vln_top_logits: bad temperature"); return VLN_ERR_ARG; }
   const vln::TopPlan p = vln::top_plan(N, V, k, type == VLN_F32 ? 4 : 8);
-  const int64_t need = vln::top_ws(p, N, k);
+  const int64_t need = vln::top_ws(p, N);
   if (need && (!ws || ws_bytes < need)) { vln::set_error("vln_top_logits: workspace too small"); return VLN_ERR_ARG; }
   vln::TopArgs a{};
   a.logits = logits; a.ld = ld; a.N = N; a.V = V; a.k = k;

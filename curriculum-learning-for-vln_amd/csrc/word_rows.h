@@ -45,6 +45,41 @@ template <typename E> __device__ __forceinline__ void st_vec(E* p, const uint4& 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, results below 2^-126 are 0
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Reductions over the wave by data-parallel moves -- row shifts of 1, 2, 4, 8 (a scan of every row of 16), then two broadcasts of row ends;
+// lane 63 holds the result -- a few cycles a step, where a shuffle through LDS takes a hundred.  The same bits in every lane.
+#define VLN_DPP(v, old, ctrl, rows) __builtin_amdgcn_update_dpp((old), (v), (ctrl), (rows), 0xf, false)
+__device__ __forceinline__ unsigned wave_umax(unsigned x) {
+  auto step = [](unsigned a, int o) { return (unsigned)o > a ? (unsigned)o : a; };
+  x = step(x, VLN_DPP((int)x, 0, 0x111, 0xf)); x = step(x, VLN_DPP((int)x, 0, 0x112, 0xf)); x = step(x, VLN_DPP((int)x, 0, 0x114, 0xf));
+  x = step(x, VLN_DPP((int)x, 0, 0x118, 0xf)); x = step(x, VLN_DPP((int)x, 0, 0x142, 0xa)); x = step(x, VLN_DPP((int)x, 0, 0x143, 0xc));
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ unsigned wave_umin(unsigned v) { return ~wave_umax(~v); }
+__device__ __forceinline__ float wave_fmax(float x) {
+  auto step = [](float a, int o) { return fmaxf(a, __int_as_float(o)); };
+  const int low = __float_as_int(-INFINITY);
+  x = step(x, VLN_DPP(__float_as_int(x), low, 0x111, 0xf)); x = step(x, VLN_DPP(__float_as_int(x), low, 0x112, 0xf));
+  x = step(x, VLN_DPP(__float_as_int(x), low, 0x114, 0xf)); x = step(x, VLN_DPP(__float_as_int(x), low, 0x118, 0xf));
+  x = step(x, VLN_DPP(__float_as_int(x), low, 0x142, 0xa)); x = step(x, VLN_DPP(__float_as_int(x), low, 0x143, 0xc));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ float wave_fsum(float x) {
+  auto step = [](float a, int o) { return a + __int_as_float(o); };
+  x = step(x, VLN_DPP(__float_as_int(x), 0, 0x111, 0xf)); x = step(x, VLN_DPP(__float_as_int(x), 0, 0x112, 0xf));
+  x = step(x, VLN_DPP(__float_as_int(x), 0, 0x114, 0xf)); x = step(x, VLN_DPP(__float_as_int(x), 0, 0x118, 0xf));
+  x = step(x, VLN_DPP(__float_as_int(x), 0, 0x142, 0xa)); x = step(x, VLN_DPP(__float_as_int(x), 0, 0x143, 0xc));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+// inclusive sum over the lanes up to this one, and the total
+__device__ __forceinline__ int wave_scan(int x, int& total) {
+  x += VLN_DPP(x, 0, 0x111, 0xf); x += VLN_DPP(x, 0, 0x112, 0xf); x += VLN_DPP(x, 0, 0x114, 0xf); x += VLN_DPP(x, 0, 0x118, 0xf);
+  x += VLN_DPP(x, 0, 0x142, 0xa); x += VLN_DPP(x, 0, 0x143, 0xc);
+  total = __builtin_amdgcn_readlane(x, 63);
+  return x;
+}
+__device__ __forceinline__ int wave_isum(int x) { int t; wave_scan(x, t); return t; }
+#undef VLN_DPP
+
 // sum_i exp((x_i - m) / T) with m = max x_i, in fp32.  m starts at the lowest FINITE value, not at -inf: x - m is then never
 // inf - inf, a row of -inf keeps sum 0 (log: -inf), and a row masked with the type's lowest value is still a distribution.
 // (x - m) is formed before the scaling: its rounding is relative to the distance, not to the logits' magnitude.
@@ -73,8 +108,8 @@ struct OnlineSum {
     m = M;
   }
   __device__ __forceinline__ void wave(float c) {      // the wave's total, the same bits in every lane
-    const float M = wave_max(m);
-    s = wave_sum(s * exp2_hw((m - M) * c));
+    const float M = wave_fmax(m);
+    s = wave_fsum(s * exp2_hw((m - M) * c));
     m = M;
   }
 };
