@@ -2,106 +2,64 @@
 // prompt, word biases, grammar masks.  include/vln_hip.h states the formula.
 //
 // Bound: bytes -- the row is read once and written once; everything per word is a handful of operations.  One workgroup takes one
-// SEGMENT of a row's columns.  How often each word of the segment stands in the history is counted into LDS (integer atomics: the
-// order does not matter), one 2-byte counter per column, so the streaming loop tests 8 columns with one 16-byte LDS read and copies
-// a vector that nothing touches.  A vector whose words are all banned is not even read, and an in-place call leaves an untouched
-// vector alone.  Every segment reads the whole history (from L2), so segments are as long as the counters allow (kSegMax) unless
-// there are too few rows to occupy the chip.
+// SEGMENT of a row's columns, up to VPT vectors of 16 bytes per thread:
+//   1. the mask bits of the thread's vectors, then the vectors that are not banned altogether, all loads in flight before anything waits;
+//   2. meanwhile how often each word of the segment stands in the history is counted into LDS (integer atomics: the order does not
+//      matter), one 2-byte counter per column, and the segment's biases are collected and summed;
+//   3. a vector's counters are one 16-byte LDS read: what nothing touches is copied (in place: left alone).
+// Every segment reads the whole history (from L2), so segments are long unless there are too few rows to occupy the chip.
 #include "word_rows.h"
 #include "../../include/vln_hip.h"
 
 namespace vln {
 
 constexpr int kCThreads = 512;
-constexpr int kSegMaxBytes = 32 * 1024;     // counters of a segment
 constexpr int kBiasMax = VLN_CONSTRAIN_MAX_BIAS;
 
 struct ConstrainArgs {
   vln_constrain a;
-  int seg_vecs;          // vectors of 16 bytes per segment
-  int n_seg;
+  int seg_vecs;          // vectors of 16 bytes per segment, <= VPT x kCThreads
+  int n_seg, xcds;       // xcds > 1: the segments of a row follow each other on one of `xcds` dies, whose L2 then serves the history
 };
 
-template <typename CT> struct Counter;      // count | flag "in the prompt" in the top bit
-template <> struct Counter<unsigned short> {
-  static constexpr unsigned kFlag = 0x8000u;
-  __device__ static __forceinline__ void count(unsigned* w, int i) { atomicAdd(&w[i >> 1], (i & 1) ? 0x10000u : 1u); }
-  __device__ static __forceinline__ void flag(unsigned* w, int i) { atomicOr(&w[i >> 1], (i & 1) ? 0x80000000u : 0x8000u); }
-  __device__ static __forceinline__ unsigned get(const unsigned* w, int i) { return (w[i >> 1] >> ((i & 1) * 16)) & 0xffffu; }
-};
-template <> struct Counter<unsigned> {
-  static constexpr unsigned kFlag = 0x80000000u;
-  __device__ static __forceinline__ void count(unsigned* w, int i) { atomicAdd(&w[i], 1u); }
-  __device__ static __forceinline__ void flag(unsigned* w, int i) { atomicOr(&w[i], kFlag); }
-  __device__ static __forceinline__ unsigned get(const unsigned* w, int i) { return w[i]; }
+// a column's counter: times in the history | "in the prompt" in the top bit | "has a bias" in the next
+template <typename CT> struct Counter {
+  static constexpr unsigned kPrompt = 1u << (8 * sizeof(CT) - 1), kBias = kPrompt >> 1, kCount = kBias - 1;
+  __device__ static __forceinline__ int shift(int i) { return sizeof(CT) == 2 ? (i & 1) * 16 : 0; }
+  __device__ static __forceinline__ unsigned* word(unsigned* w, int i) { return &w[sizeof(CT) == 2 ? i >> 1 : i]; }
+  __device__ static __forceinline__ void count(unsigned* w, int i) { atomicAdd(word(w, i), 1u << shift(i)); }
+  __device__ static __forceinline__ bool flag(unsigned* w, int i, unsigned bit) { return (atomicOr(word(w, i), bit << shift(i)) >> shift(i)) & bit; }
+  __device__ static __forceinline__ unsigned get(unsigned* w, int i) { return sizeof(CT) == 2 ? (*word(w, i) >> shift(i)) & 0xffffu : *word(w, i); }
 };
 
 struct Penalty { float r, p, f; };
 
 template <typename CT> __device__ __forceinline__ float penalised(float z, unsigned n, const Penalty& q) {
-  if (n) z = z > 0.f ? z / q.r : z * q.r;
-  const unsigned c = n & ~Counter<CT>::kFlag;
+  typedef Counter<CT> Cn;
+  if (n & (Cn::kPrompt | Cn::kCount)) z = z > 0.f ? z / q.r : z * q.r;
+  const unsigned c = n & Cn::kCount;
   if (c) z -= q.f * (float)c + q.p;
   return z;
 }
 
 // E: logits; CT: counter; BWD: in = d out, out = d logits, `logits` = the forward's input (its sign decides the repetition factor)
-template <typename E, typename CT, bool BWD>
-__global__ __launch_bounds__(kCThreads) void constrain_kernel(ConstrainArgs k) {
+template <typename E, typename CT, int VPT, bool BWD>
+// (four workgroups per CU: 96 scalar registers, 64 vector registers)
+__global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) void constrain_kernel(ConstrainArgs k) {
   extern __shared__ unsigned lds[];
   const vln_constrain& a = k.a;
   constexpr int VEC = RowGeo<E>::VEC;
+  constexpr unsigned all = (1u << VEC) - 1u;
   typedef Counter<CT> Cn;
-  const int b = blockIdx.x, seg = blockIdx.y, tid = threadIdx.x;
+  const int turn = blockIdx.x / k.xcds, tid = threadIdx.x;
+  const int b = turn / k.n_seg * k.xcds + blockIdx.x % k.xcds, seg = turn % k.n_seg;
+  if (b >= a.B) return;
   const E* in = static_cast<const E*>(a.in) + (int64_t)b * a.ld_in;
   const E* zr = BWD ? static_cast<const E*>(a.logits) + (int64_t)b * a.ld_logits : in;
   E* out = static_cast<E*>(a.out) + (int64_t)b * a.ld_out;
   const RowGeo<E> g(in, a.V);
-  const int v0 = seg * k.seg_vecs, v1 = min(g.nv, v0 + k.seg_vecs);
-  // Counter slots: the segment's vectors in order, then (first segment only) the single columns of head and tail.
-  const int nslot_v = k.seg_vecs * VEC;
-  auto slot = [&](long id) -> int {
-    if (id < 0 || id >= a.V) return -1;
-    const int c = (int)id;
-    if (c < g.head) return seg == 0 ? nslot_v + c : -1;
-    if (c >= g.tail0()) return seg == 0 ? nslot_v + VEC + (c - g.tail0()) : -1;
-    const int i = c - g.head - v0 * VEC;
-    return (i >= 0 && i < (v1 - v0) * VEC) ? i : -1;
-  };
-  const int nslots = nslot_v + 2 * VEC;
-  const int nwords = (nslots * (int)sizeof(CT) + 15) / 16 * 4;
-  for (int i = tid; i < nwords / 4; i += kCThreads) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
-  __shared__ int n_here;
-  if (tid == 0) n_here = 0;
-  __syncthreads();
-  const long hl = a.history ? (a.history_len ? min((long)a.history_len[b], (long)a.H) : (long)a.H) : 0;
-  for (long i = tid; i < hl; i += kCThreads) {
-    const int s = slot(a.history[(int64_t)b * a.ld_history + i]);
-    if (s >= 0) Cn::count(lds, s);
-  }
-  const long pl = a.prompt ? (a.prompt_len ? min((long)a.prompt_len[b], (long)a.P) : (long)a.P) : 0;
-  for (long i = tid; i < pl; i += kCThreads) {
-    const int s = slot(a.prompt[(int64_t)b * a.ld_prompt + i]);
-    if (s >= 0) Cn::flag(lds, s);
-  }
-  // The segment's bias entries: {slot, entry} pairs and the logit as it is before any of this row is written (in-place calls).
-  int* b_slot = reinterpret_cast<int*>(lds + nwords);
-  int* b_entry = b_slot + a.n_bias;
-  float* b_z = reinterpret_cast<float*>(b_entry + a.n_bias);
-  if (!BWD && a.n_bias) {
-    for (int j = tid; j < a.n_bias; j += kCThreads) {
-      const long id = a.bias_ids[(int64_t)b * a.ld_bias_ids + j];
-      const int s = slot(id);
-      if (s >= 0) {
-        const int at = atomicAdd(&n_here, 1);
-        b_slot[at] = s; b_entry[at] = j; b_z[at] = Elt<E>::ld(in + id);
-      }
-    }
-  }
-  __syncthreads();
-
-  const Penalty q{a.repetition ? a.repetition[b] : a.repetition_all, a.presence ? a.presence[b] : a.presence_all,
-                  a.frequency ? a.frequency[b] : a.frequency_all};
+  const int v0 = min(g.nv, seg * k.seg_vecs), v1 = min(g.nv, v0 + k.seg_vecs);
+  const bool in_place = !BWD && static_cast<const void*>(in) == static_cast<const void*>(out);
   // mask row: NULL = every word allowed; a row index outside [-1, G) bans every word (the grammar did not allow any)
   const unsigned* mk = nullptr;
   bool ban_all = false;
@@ -112,7 +70,6 @@ __global__ __launch_bounds__(kCThreads) void constrain_kernel(ConstrainArgs k) {
   }
   const int last_word = (a.V - 1) >> 5;
   auto bits_at = [&](int c) -> unsigned {       // VEC mask bits of columns c .. c + VEC - 1
-    constexpr unsigned all = (1u << VEC) - 1u;
     if (ban_all) return 0u;
     if (!mk) return all;
     const int w = c >> 5, sh = c & 31;
@@ -120,95 +77,196 @@ __global__ __launch_bounds__(kCThreads) void constrain_kernel(ConstrainArgs k) {
     if (sh + VEC > 32 && w < last_word) x |= mk[w + 1] << (32 - sh);
     return x & all;
   };
+  // What the counting needs is asked for first (loads come back in order), then the mask bits, then the logits.
+  constexpr int HP = 8;
+  const int64_t* hist = a.history + (int64_t)b * a.ld_history;
+  int64_t first_ids[HP];
+#pragma unroll
+  for (int t = 0; t < HP; ++t) first_ids[t] = t * kCThreads + tid < a.H ? hist[t * kCThreads + tid] : -1;
+  int64_t bias_id = -1;
+  float bias_val = 0.f;
+  if (!BWD && tid < a.n_bias) {
+    bias_id = a.bias_ids[(int64_t)b * a.ld_bias_ids + tid];
+    bias_val = a.bias_values[(int64_t)b * a.ld_bias_values + tid];
+  }
+  unsigned ok[VPT];
+  uint4 raw[VPT];
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {
+    const int i = v0 + u * kCThreads + tid;
+    ok[u] = i < v1 ? bits_at(g.head + i * VEC) : 0u;
+  }
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {
+    raw[u] = make_uint4(0, 0, 0, 0);
+    if (ok[u] && !in_place) raw[u] = ld_vec<E>(in + g.head + (int64_t)(v0 + u * kCThreads + tid) * VEC);
+  }
+
+  // Counter slots: the segment's vectors in order, then (first segment only) the single columns of head and tail.
+  const int nslot_v = k.seg_vecs * VEC, col0 = g.head + v0 * VEC, cols = (v1 - v0) * VEC;
+  auto slot = [&](int64_t id) -> int {
+    const int64_t i = id - col0;
+    if (i >= 0 && i < cols) return (int)i;
+    if (seg != 0) return -1;
+    if (id >= 0 && id < g.head) return nslot_v + (int)id;
+    if (id >= g.tail0() && id < a.V) return nslot_v + VEC + (int)(id - g.tail0());
+    return -1;
+  };
+  const int nwords = ((nslot_v + 2 * VEC) * (int)sizeof(CT) + 15) / 16 * 4;
+  for (int i = tid; i < nwords / 4; i += kCThreads) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+  __shared__ int n_here, n_twice;
+  if (tid == 0) n_here = n_twice = 0;
+  __syncthreads();
+  auto length = [&](const int64_t* lens, int n) { return (int)(lens ? max((int64_t)0, min(lens[b], (int64_t)n)) : (int64_t)n); };
+  const int hl = length(a.history_len, a.H);
+#pragma unroll
+  for (int t = 0; t < HP; ++t) {
+    const int s = t * kCThreads + tid < hl ? slot(first_ids[t]) : -1;
+    if (s >= 0) Cn::count(lds, s);
+  }
+  auto each = [&](const int64_t* row, int from, int len, auto&& f) {      // the ids that fall into this segment
+    for (int i = from + tid; i < len; i += 4 * kCThreads) {
+      int64_t id[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) id[t] = i + t * kCThreads < len ? row[i + t * kCThreads] : -1;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int s = slot(id[t]);
+        if (s >= 0) f(s);
+      }
+    }
+  };
+  each(hist, HP * kCThreads, hl, [&](int s) { Cn::count(lds, s); });
+  if (a.P) each(a.prompt + (int64_t)b * a.ld_prompt, 0, length(a.prompt_len, a.P), [&](int s) { Cn::flag(lds, s, Cn::kPrompt); });
+  // The segment's bias entries: slot, entry, value and the logit as it is before any of this row is written (in-place calls).
+  int4* bias = reinterpret_cast<int4*>(lds + nwords);
+  if (!BWD) {
+    for (int j = tid; j < a.n_bias; j += kCThreads) {
+      if (j != tid) {
+        bias_id = a.bias_ids[(int64_t)b * a.ld_bias_ids + j];
+        bias_val = a.bias_values[(int64_t)b * a.ld_bias_values + j];
+      }
+      const int s = slot(bias_id);
+      if (s >= 0) {
+        const float z = (bits_at((int)bias_id) & 1u) ? Elt<E>::ld(in + bias_id) : -INFINITY;
+        bias[atomicAdd(&n_here, 1)] = make_int4(s, j, __float_as_int(bias_val), __float_as_int(z));
+        if (Cn::flag(lds, s, Cn::kBias)) n_twice = 1;
+      }
+    }
+  }
+  __syncthreads();
+
+  const Penalty q{a.repetition ? a.repetition[b] : a.repetition_all, a.presence ? a.presence[b] : a.presence_all,
+                  a.frequency ? a.frequency[b] : a.frequency_all};
+  // A word's biases are added up in entry order by its FIRST entry: the same bits whatever order the entries were collected in.
+  constexpr int BPT = kBiasMax / kCThreads;
+  int b_col[BPT];
+  float b_out[BPT];
+  const int nb = n_here;
+  if (!BWD && nb) {
+#pragma unroll
+    for (int t = 0; t < BPT; ++t) {
+      b_col[t] = -1;
+      const int j = t * kCThreads + tid;
+      if (j >= nb) continue;
+      const int4 me = bias[j];
+      float sum = __int_as_float(me.z);
+      if (n_twice) {                              // some word of the segment has more than one entry
+        int same = 0;
+        bool first = true;
+        for (int i = 0; i < nb; ++i) {
+          const int2 o = *reinterpret_cast<const int2*>(&bias[i]);
+          same += o.x == me.x ? 1 : 0;
+          first = first && !(o.x == me.x && o.y < me.y);
+        }
+        if (!first) continue;
+        for (int prev = me.y; --same > 0;) {
+          int next = 0x7fffffff, at = 0;
+          for (int i = 0; i < nb; ++i) if (bias[i].x == me.x && bias[i].y > prev && bias[i].y < next) { next = bias[i].y; at = i; }
+          sum += __int_as_float(bias[at].z);
+          prev = next;
+        }
+      }
+      const int s = me.x;
+      b_col[t] = s < nslot_v ? col0 + s : (s < nslot_v + VEC ? s - nslot_v : g.tail0() + s - nslot_v - VEC);
+      b_out[t] = penalised<CT>(__int_as_float(me.w), Cn::get(lds, s), q) + sum;
+      if (!(bits_at(b_col[t]) & 1u)) b_out[t] = -INFINITY;
+    }
+  }
   const float banned = BWD ? 0.f : -INFINITY;
   auto one = [&](float x, unsigned n, int c) -> float {          // one allowed column
     if (!BWD) return penalised<CT>(x, n, q);
-    if (!n) return x;
+    if (!(n & (Cn::kPrompt | Cn::kCount))) return x;
     return Elt<E>::ld(zr + c) > 0.f ? x / q.r : x * q.r;
   };
   auto single = [&](int c, int s) {
-    const bool ok = bits_at(c) & 1u;
-    Elt<E>::st(out + c, ok ? one(Elt<E>::ld(in + c), Cn::get(lds, s), c) : banned);
+    const bool may = bits_at(c) & 1u;
+    Elt<E>::st(out + c, may ? one(Elt<E>::ld(in + c), Cn::get(lds, s), c) : banned);
   };
   if (seg == 0) {
     if (tid < g.head) single(tid, nslot_v + tid);
     else if (tid >= VEC && tid - VEC < g.tail) single(g.tail0() + tid - VEC, nslot_v + tid);
   }
-  const bool in_place = !BWD && static_cast<const void*>(in) == static_cast<const void*>(out);
   const bool vec_out = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  for (int i = v0 + tid; i < v1; i += kCThreads) {
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {
+    const int i = v0 + u * kCThreads + tid;
+    if (i >= v1) continue;
     const int c = g.head + i * VEC, s = (i - v0) * VEC;
     constexpr int CW = VEC * (int)sizeof(CT) / 4;      // counter words of a vector: 2 or 4 (u16), 4 or 8 (u32)
     unsigned cw[CW], any = 0;
 #pragma unroll
     for (int w = 0; w < CW; ++w) { cw[w] = lds[s * (int)sizeof(CT) / 4 + w]; any |= cw[w]; }
-    const unsigned ok = bits_at(c);
-    constexpr unsigned all = (1u << VEC) - 1u;
-    if (in_place && ok == all && !any) continue;
+    if (in_place) {
+      if (ok[u] == all && !any) continue;
+      if (ok[u]) raw[u] = ld_vec<E>(in + c);
+    }
     float x[VEC];
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (ok) raw = ld_vec<E>(in + c);
-    if (ok != all || any) {
-      unpack16<E>(raw, x);
+    if (ok[u] != all || any) {
+      unpack16<E>(raw[u], x);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const unsigned n = sizeof(CT) == 2 ? (cw[j / 2] >> ((j & 1) * 16)) & 0xffffu : cw[j * CW / VEC];
-        x[j] = ((ok >> j) & 1u) ? (n ? one(x[j], n, c + j) : x[j]) : banned;
+        x[j] = ((ok[u] >> j) & 1u) ? (n ? one(x[j], n, c + j) : x[j]) : banned;
       }
-      raw = pack16<E>(x);
+      raw[u] = pack16<E>(x);
     }
     if (vec_out) {
-      st_vec<E>(out + c, raw);
+      st_vec<E>(out + c, raw[u]);
     } else {
-      unpack16<E>(raw, x);
+      unpack16<E>(raw[u], x);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) Elt<E>::st(out + c + j, x[j]);
     }
   }
-  if (BWD || !a.n_bias) return;
+  if (BWD || !nb) return;
   __syncthreads();
-  // A word's biases are added up in entry order by its FIRST entry: the same bits whatever order the entries were collected in.
-  const int n = n_here;
-  for (int j = tid; j < n; j += kCThreads) {
-    const int s = b_slot[j], e = b_entry[j];
-    bool first = true;
-    for (int i = 0; i < n; ++i) first = first && !(b_slot[i] == s && b_entry[i] < e);
-    if (!first) continue;
-    float sum = 0.f;
-    int prev = e - 1;
-    while (true) {
-      int next = 0x7fffffff;
-      for (int i = 0; i < n; ++i) if (b_slot[i] == s && b_entry[i] > prev) next = min(next, b_entry[i]);
-      if (next == 0x7fffffff) break;
-      sum += a.bias_values[(int64_t)b * a.ld_bias_values + next];
-      prev = next;
-    }
-    const int c = (int)a.bias_ids[(int64_t)b * a.ld_bias_ids + e];
-    if (bits_at(c) & 1u) Elt<E>::st(out + c, penalised<CT>(b_z[j], Cn::get(lds, s), q) + sum);
-  }
+#pragma unroll
+  for (int t = 0; t < BPT; ++t) if (t * kCThreads + tid < nb && b_col[t] >= 0) Elt<E>::st(out + b_col[t], b_out[t]);
 }
 
-template <typename E, typename CT> static int constrain_launch(const vln_constrain& a, hipStream_t st) {
+template <typename E, typename CT, int VPT> static int constrain_launch(const vln_constrain& a, hipStream_t st) {
   constexpr int VEC = Elt<E>::kVec;
   ConstrainArgs k;
   k.a = a;
   const int nv = (a.V + VEC - 1) / VEC;
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  const int per_seg_max = kSegMaxBytes / (int)sizeof(CT) / VEC;             // vectors whose counters fit
-  int n_seg = (nv + per_seg_max - 1) / per_seg_max;
+  int n_seg = (nv + VPT * kCThreads - 1) / (VPT * kCThreads);
   const int want = (2 * cus + a.B - 1) / a.B;                               // two workgroups per CU ...
   const int finest = (nv + kCThreads - 1) / kCThreads;                      // ... but at least a vector per thread
   if (n_seg < want) n_seg = want < finest ? want : finest;
-  if (n_seg < 1) n_seg = 1;
+  const size_t lists = a.backward ? 0 : (size_t)a.n_bias * 16;
+  const int fits = (int)((65536 - 64 - lists) / sizeof(CT)) / VEC - 2;      // 64 KB of LDS with the bias lists
   k.seg_vecs = (nv + n_seg - 1) / n_seg;
-  if (k.seg_vecs < 1) k.seg_vecs = 1;
+  if (k.seg_vecs > fits) k.seg_vecs = fits;
   k.n_seg = (nv + k.seg_vecs - 1) / k.seg_vecs;
-  if (k.n_seg < 1) k.n_seg = 1;
-  const int slots = k.seg_vecs * VEC + 2 * VEC;
-  const unsigned lds = (unsigned)((slots * sizeof(CT) + 15) / 16 * 16 + (a.backward ? 0 : (size_t)a.n_bias * 12));
-  const dim3 grid((unsigned)a.B, (unsigned)k.n_seg);
-  if (a.backward) VLN_LAUNCH((constrain_kernel<E, CT, true>), grid, dim3(kCThreads), lds, st, k);
-  else VLN_LAUNCH((constrain_kernel<E, CT, false>), grid, dim3(kCThreads), lds, st, k);
+  // Workgroups go to the 8 dies in turn.  With rows enough for all dies the segments of a row share one (the history comes from memory
+  // once: 512 rows x 131072 bf16, 4096 words of history: see below); with few rows they spread over all.
+  k.xcds = a.B >= 64 ? 8 : 1;
+  const unsigned lds = (unsigned)(((k.seg_vecs * VEC + 2 * VEC) * sizeof(CT) + 15) / 16 * 16 + lists);
+  const dim3 grid((unsigned)((a.B + k.xcds - 1) / k.xcds * k.xcds * k.n_seg));
+  if (a.backward) VLN_LAUNCH((constrain_kernel<E, CT, VPT, true>), grid, dim3(kCThreads), lds, st, k);
+  else VLN_LAUNCH((constrain_kernel<E, CT, VPT, false>), grid, dim3(kCThreads), lds, st, k);
   VLN_CHECK_LAUNCH("constrain_logits");
   return VLN_OK;
 }
@@ -229,9 +287,10 @@ extern "C" int vln_constrain_logits(const vln_constrain* p, vln_stream_t s) {
     vln::set_error("vln_constrain_logits: bad mask"); return VLN_ERR_ARG;
   }
   hipStream_t st = (hipStream_t)s;
-  const bool small = a.H < 0x8000;          // 15 bits of count
-  if (a.type == VLN_F32) return small ? vln::constrain_launch<float, unsigned short>(a, st) : vln::constrain_launch<float, unsigned>(a, st);
-  if (a.type == VLN_BF16) return small ? vln::constrain_launch<bf16_raw, unsigned short>(a, st) : vln::constrain_launch<bf16_raw, unsigned>(a, st);
+  const bool small = a.H < 0x4000;          // 14 bits of count
+  // (LDS of a segment: 32 KB of counters at most, and 16 bytes per bias of the row)
+  if (a.type == VLN_F32) return small ? vln::constrain_launch<float, unsigned short, 4>(a, st) : vln::constrain_launch<float, unsigned, 4>(a, st);
+  if (a.type == VLN_BF16) return small ? vln::constrain_launch<bf16_raw, unsigned short, 4>(a, st) : vln::constrain_launch<bf16_raw, unsigned, 2>(a, st);
   vln::set_error("vln_constrain_logits: type must be fp32 or bf16");
   return VLN_ERR_ARG;
 }

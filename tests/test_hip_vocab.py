@@ -135,7 +135,8 @@ def constrain_tol(dt, ref, scale, nb):
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 @pytest.mark.parametrize("how", ["plain", "wide", "odd"])
 @pytest.mark.parametrize("N,V,H,P,nb,grammar", [(1, 1, 1, 1, 1, False), (3, 7, 5, 0, 3, True), (4, 31, 40, 9, 20, True), (5, 64, 0, 0, 0, True),
-                                                (2, 992, 80, 30, 0, False), (6, 1003, 300, 40, 200, True), (3, 20011, 700, 100, 50, True)])
+                                                (2, 992, 80, 30, 0, False), (6, 1003, 300, 40, 200, True), (3, 20011, 700, 100, 50, True),
+                                                (2, 40000, 9000, 5000, 2048, False)])
 def test_constrain_logits(vocab, N, V, H, P, nb, grammar, how, dt):
     c, ref = constrain_case(N, V, H, P, nb, grammar, 7 * N + V + H)
     g = torch.Generator().manual_seed(V)
@@ -182,9 +183,9 @@ def test_constrain_gradient_against_differences(vocab):
     close(dz, num, 2 * U * num.abs() + 1e-9, "d logits")
 
 
-@pytest.mark.parametrize("H", [32767, 32768, 70000])
+@pytest.mark.parametrize("H", [16383, 16384, 32767, 32768, 70000])
 def test_constrain_long_histories(vocab, H):
-    """One word all the time: counts on both sides of the 15-bit counters, and past 16 bits."""
+    """One word all the time: counts on both sides of the 14- and 15-bit counters, and past 16 bits."""
     V = 40
     z = torch.ones(2, V, device=dev())
     hist = torch.full((2, H), 5, dtype=torch.int64, device=dev())
