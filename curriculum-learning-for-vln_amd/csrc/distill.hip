@@ -8,6 +8,8 @@
 // keep (a bitmap of the kept ones in LDS, one byte tested per 8 logits): the mass of the others is a sum of positive terms, never
 // 1 - (sum of the kept), which cancels when the student is sure.  The kept words (<= VLN_DISTILL_MAX per row) are handled by their own
 // lanes: loss terms in the forward, and in the backward their gradients overwrite what the streaming loop wrote there.
+#include <type_traits>
+
 #include "word_rows.h"
 #include "../../include/vln_hip.h"
 
@@ -24,7 +26,7 @@ struct DistillArgs {
   const float* t_rest;
   const long long* target;
   long ignore;
-  int N, V, K, S, seg_vecs;
+  int N, V, K, W, S, seg_vecs;
   float c, invT, T, alpha;
   float* rows; float* stats;
   float4* part;               // S > 1: [N, S]
@@ -56,12 +58,12 @@ template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(cons
   auto outcome = [&](float u) { tm = fmaxf(tm, u); nan = nan || u != u; };
   if (TAIL) outcome(a.t_rest[n]);
   for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) outcome(teacher_u(a, n, j));
-  tm = wave_max(tm);
+  tm = wave_fmax(tm);
   const bool soft = tm != -INFINITY || __any(nan);
   const float tref = tm != -INFINITY ? tm : 0.f;
   float ts = 0.f;
   for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) ts += exp2_hw((teacher_u(a, n, j) - tref) * kLog2e);
-  ts = wave_sum(ts);
+  ts = wave_fsum(ts);
   const float er = TAIL ? exp2_hw((a.t_rest[n] - tref) * kLog2e) : 0.f;
   ts += er;
   // a word listed twice: only its first entry counts in the student's total
@@ -76,7 +78,7 @@ template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(cons
   if (TAIL) {
     float M = dense.m;
     for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) M = fmaxf(M, Elt<E>::ld(p + kid[j]));
-    M = wave_max(M);
+    M = wave_fmax(M);
     float t = 0.f, t1 = 0.f;
     for (int j = lane; j < a.K; j += 64) {
       const int id = kid[j];
@@ -88,8 +90,8 @@ template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(cons
         t1 += exp2_hw(d * kLog2e);
       }
     }
-    all.s = dense.s * exp2_hw((dense.m - M) * c) + wave_sum(t);
-    s1 = s1 * exp2_hw((dense.m - M) * kLog2e) + wave_sum(t1);
+    all.s = dense.s * exp2_hw((dense.m - M) * c) + wave_fsum(t);
+    s1 = s1 * exp2_hw((dense.m - M) * kLog2e) + wave_fsum(t1);
     all.m = M;
   }
   const float log_s = logf(all.s), log_ts = logf(ts);
@@ -109,7 +111,7 @@ template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(cons
       loss += exp2_hw(lr * kLog2e) * (lr - lpr);
     }
   }
-  loss = wave_sum(loss) * a.alpha * a.T * a.T;
+  loss = wave_fsum(loss) * a.alpha * a.T * a.T;
   if (a.alpha == 0.f) loss = 0.f;
   const bool live = a.target ? !row_ignored(a, n) : soft;
   if (a.target && a.alpha < 1.f) {
@@ -130,33 +132,47 @@ template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(cons
 __device__ __forceinline__ void dead_row(const DistillArgs& a, long n, int lane) {
   if (lane == 0) { a.rows[n] = 0.f; a.stats[n * kStat + ST_FLAGS] = __int_as_float(0); }
 }
-__device__ __forceinline__ void stage_ids(const DistillArgs& a, long n, int* kid, int lane) {
-  for (int j = lane; j < a.K; j += 64) {
+// one wave joins the (maximum, sum at T, sum at 1) of `count` parts, in their order per lane
+__device__ __forceinline__ void join_parts(OnlineSum& o, float& s1, const float4* parts, int count, float c, int lane) {
+  o = OnlineSum();
+  s1 = 0.f;
+  for (int i = lane; i < count; i += 64) {
+    const float4 q = parts[i];
+    const float M = fmaxf(o.m, q.x);
+    s1 = s1 * exp2_hw((o.m - M) * kLog2e) + q.z * exp2_hw((q.x - M) * kLog2e);
+    o.merge(q.x, q.y, c);
+  }
+  const float M = wave_fmax(o.m);
+  s1 = wave_fsum(s1 * exp2_hw((o.m - M) * kLog2e));
+  o.wave(c);
+}
+template <int B> __device__ __forceinline__ void stage_ids(const DistillArgs& a, long n, int* kid, int tid) {
+  for (int j = tid; j < a.K; j += B) {
     const long long id = a.ids[n * a.ld_ids + j];
     kid[j] = (id >= 0 && id < a.V) ? (int)id : -1;
   }
   __syncthreads();
 }
 
-// HARD: also the sum at temperature 1 (T != 1 and a hard target); otherwise s1 is the sum at T.
-template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) void distill_fwd_kernel(DistillArgs a) {
+// HARD: also the sum at temperature 1 (T != 1 and a hard target); otherwise s1 is the sum at T.  W: waves of a row (or segment).
+template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(64 * W) void distill_fwd_kernel(DistillArgs a) {
   extern __shared__ unsigned lds[];
-  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC;
+  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC, B = 64 * W;
   const long n = blockIdx.x;
-  const int s = blockIdx.y, lane = threadIdx.x;
-  if (row_ignored(a, n)) { if (s == 0) dead_row(a, n, lane); return; }
+  const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (row_ignored(a, n)) { if (s == 0) dead_row(a, n, tid); return; }
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   const RowGeo<E> g(p, a.V);
   const int v0 = min(g.nv, s * a.seg_vecs), v1 = min(g.nv, v0 + a.seg_vecs);
   int* kid = reinterpret_cast<int*>(lds);
   unsigned* bm = lds + (a.K + 3) / 4 * 4;        // bit i: column i of the segment's vectors; then head, then tail (VEC bits each)
   const int nbits_v = a.seg_vecs * VEC;
-  if (TAIL || a.S == 1) stage_ids(a, n, kid, lane);
+  if (TAIL || a.S == 1) stage_ids<B>(a, n, kid, tid);
   if (TAIL) {
     const int nw = (nbits_v + 2 * VEC + 31) / 32;
-    for (int i = lane; i < nw; i += 64) bm[i] = 0u;
+    for (int i = tid; i < nw; i += B) bm[i] = 0u;
     __syncthreads();
-    for (int j = lane; j < a.K; j += 64) {
+    for (int j = tid; j < a.K; j += B) {
       const int id = kid[j];
       if (id < 0) continue;
       int bit = -1;
@@ -187,23 +203,23 @@ template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) voi
   };
   if (s == 0) {
     int col = -1, bit = 0;
-    if (lane < g.head) { col = lane; bit = nbits_v + lane; }
-    else if (lane >= VEC && lane - VEC < g.tail) { col = g.tail0() + lane - VEC; bit = nbits_v + lane; }
+    if (tid < g.head) { col = tid; bit = nbits_v + tid; }
+    else if (tid >= VEC && tid - VEC < g.tail) { col = g.tail0() + tid - VEC; bit = nbits_v + tid; }
     float x[1] = {col >= 0 ? Elt<E>::ld(p + col) : -INFINITY};
     if (TAIL && col >= 0 && ((bm[bit >> 5] >> (bit & 31)) & 1u)) x[0] = -INFINITY;
     take(x, x[0]);
   }
-  for (int v = v0 + lane; v < v1; v += 64 * U) {
+  for (int v = v0 + tid; v < v1; v += B * U) {
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * 64, v1 - 1) * VEC);
+    for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * B, v1 - 1) * VEC);
     float x[16];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       unpack16<E>(raw[u], x + u * VEC);
       unsigned out = 0u;             // bit j: element j does not count
-      if (TAIL) { const int bit = (v + u * 64 - v0) * VEC; if (v + u * 64 < v1) out = (bm[bit >> 5] >> (bit & 31)) & ((1u << VEC) - 1u); }
-      if (v + u * 64 >= v1) out = ~0u;
+      if (TAIL) { const int bit = (v + u * B - v0) * VEC; if (v + u * B < v1) out = (bm[bit >> 5] >> (bit & 31)) & ((1u << VEC) - 1u); }
+      if (v + u * B >= v1) out = ~0u;
       if (out) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) if ((out >> j) & 1u) x[u * VEC + j] = -INFINITY;
@@ -214,12 +230,18 @@ template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) voi
     for (int j = 1; j < 16; ++j) mx = fmaxf(mx, x[j]);
     take(x, mx);
   }
-  // the wave's total
-  const float M = wave_max(o.m);
-  if (HARD) s1 = wave_sum(s1 * exp2_hw((o.m - M) * kLog2e));
-  o.s = wave_sum(o.s * exp2_hw((o.m - M) * a.c));
+  const float M = wave_fmax(o.m);
+  if (HARD) s1 = wave_fsum(s1 * exp2_hw((o.m - M) * kLog2e));
+  o.s = wave_fsum(o.s * exp2_hw((o.m - M) * a.c));
   o.m = M;
   if (!HARD) s1 = o.s;
+  if (W > 1) {
+    __shared__ float4 parts[W];
+    if (lane == 0) parts[w] = make_float4(o.m, o.s, s1, 0.f);
+    __syncthreads();
+    if (w > 0) return;
+    join_parts(o, s1, parts, W, a.c, lane);
+  }
   if (a.S == 1) finish_row<E, TAIL>(a, n, o, s1, kid, lane);
   else if (lane == 0) a.part[n * a.S + s] = make_float4(o.m, o.s, s1, 0.f);
 }
@@ -230,18 +252,10 @@ template <typename E, bool TAIL> __global__ __launch_bounds__(64) void distill_j
   const int lane = threadIdx.x;
   if (row_ignored(a, n)) return;
   int* kid = reinterpret_cast<int*>(lds);
-  stage_ids(a, n, kid, lane);
+  stage_ids<64>(a, n, kid, lane);
   OnlineSum o;
-  float s1 = 0.f;
-  for (int i = lane; i < a.S; i += 64) {
-    const float4 q = a.part[n * a.S + i];
-    const float M = fmaxf(o.m, q.x);
-    s1 = s1 * exp2_hw((o.m - M) * kLog2e) + q.z * exp2_hw((q.x - M) * kLog2e);
-    o.merge(q.x, q.y, a.c);
-  }
-  const float M = wave_max(o.m);
-  s1 = wave_sum(s1 * exp2_hw((o.m - M) * kLog2e));
-  o.wave(a.c);
+  float s1;
+  join_parts(o, s1, a.part + n * a.S, a.S, a.c, lane);
   finish_row<E, TAIL>(a, n, o, s1, kid, lane);
 }
 
@@ -255,7 +269,7 @@ __global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows,
     acc += rows[i];
     n += __float_as_int(stats[(long)i * kStat + ST_FLAGS]) & ROW_LIVE;
   }
-  acc = wave_sum(acc);
+  acc = wave_fsum(acc);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
   if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = acc; cnt[threadIdx.x >> 6] = n; }
@@ -272,11 +286,13 @@ __global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows,
 // d z_v = g [ alpha T (p_v - q_v) + (1 - alpha) (softmax(z)_v - [v = y]) ], p_v - r p_v / p_rest for the words the teacher did not keep.
 // The streaming loop evaluates  A exp((z - M) / T) + H exp(z - M)  with one pair (A, H) per row: M is the maximum the exponentials of
 // that loop are bounded by (TAIL: the others' maximum), so neither a sure student's tiny p_rest nor its kept words leave the range.
-template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) void distill_bwd_kernel(DistillArgs a) {
+template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(64 * W) void distill_bwd_kernel(DistillArgs a) {
   extern __shared__ unsigned lds[];
-  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC;
+  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC, B = 64 * W;
+  __shared__ int y_kept;
   const long n = blockIdx.x;
-  const int s = blockIdx.y, lane = threadIdx.x;
+  const int s = blockIdx.y, tid = threadIdx.x;
+  if (tid == 0) y_kept = 0;
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   E* dz = static_cast<E*>(a.dz) + n * a.ldz;
   const float* st = a.stats + n * kStat;
@@ -284,11 +300,11 @@ template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) voi
   const RowGeo<E> g(dz, a.V);                 // the writes decide the alignment
   const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
   const int v0 = min(g.nv, s * a.seg_vecs), v1 = min(g.nv, v0 + a.seg_vecs);
-  const bool single = s == 0 && (lane < g.head || (lane >= VEC && lane - VEC < g.tail));
-  const int scol = lane < g.head ? lane : g.tail0() + lane - VEC;
+  const bool single = s == 0 && (tid < g.head || (tid >= VEC && tid - VEC < g.tail));
+  const int scol = tid < g.head ? tid : g.tail0() + tid - VEC;
   if (!(flags & ROW_LIVE)) {                  // an ignored row: zeros, whatever its logits hold
     if (single) Elt<E>::st(dz + scol, 0.f);
-    for (int v = v0 + lane; v < v1; v += 64) st_vec<E>(dz + g.head + (int64_t)v * VEC, make_uint4(0, 0, 0, 0));
+    for (int v = v0 + tid; v < v1; v += B) st_vec<E>(dz + g.head + (int64_t)v * VEC, make_uint4(0, 0, 0, 0));
     return;
   }
   const float up = a.g[n * a.g_stride] * (a.inv_count ? a.inv_count[0] : 1.f);
@@ -313,26 +329,26 @@ template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) voi
   };
   if (single) Elt<E>::st(dz + scol, grad(Elt<E>::ld(p + scol)));
   if (same) {
-    for (int v = v0 + lane; v < v1; v += 64 * U) {
+    for (int v = v0 + tid; v < v1; v += B * U) {
       uint4 raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * 64, v1 - 1) * VEC);
+      for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * B, v1 - 1) * VEC);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float x[VEC];
         unpack16<E>(raw[u], x);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) x[j] = grad(x[j]);
-        if (v + u * 64 < v1) st_vec<E>(dz + g.head + (int64_t)(v + u * 64) * VEC, pack16<E>(x));
+        if (v + u * B < v1) st_vec<E>(dz + g.head + (int64_t)(v + u * B) * VEC, pack16<E>(x));
       }
     }
   } else {                                    // rows that start at different distances from a 16-byte boundary
-    for (int c = g.head + v0 * VEC + lane; c < g.head + v1 * VEC; c += 64) Elt<E>::st(dz + c, grad(Elt<E>::ld(p + c)));
+    for (int c = g.head + v0 * VEC + tid; c < g.head + v1 * VEC; c += B) Elt<E>::st(dz + c, grad(Elt<E>::ld(p + c)));
   }
   // the kept words and the target: their own values over what the loop wrote
   int* kid = reinterpret_cast<int*>(lds);
   const int nk = soft || TAIL ? a.K : 0;
-  if (nk) stage_ids(a, n, kid, lane); else __syncthreads();
+  if (nk) stage_ids<B>(a, n, kid, tid); else __syncthreads();
   auto mine = [&](long id) {
     if (id < g.head || id >= g.tail0()) return s == 0;
     const int i = (int)((id - g.head) / VEC);
@@ -345,11 +361,10 @@ template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) voi
     if (hard) v += gh * (exp2_hw(d * kLog2e) * is1 - (id == y ? 1.f : 0.f));
     return bad_y ? __builtin_nanf("") : v;
   };
-  bool y_kept = false;
-  for (int j = lane; j < nk; j += 64) {
+  for (int j = tid; j < nk; j += B) {
     const int id = kid[j];
     if (id < 0) continue;
-    y_kept = y_kept || id == y;
+    if (id == y) y_kept = 1;
     if (!mine(id)) continue;
     float q = soft ? exp2_hw((teacher_u(a, n, j) - tm) * kLog2e) * its : 0.f;
     if (soft && (flags & ROW_TWICE)) {                  // listed more than once: the first entry writes the sum, in entry order
@@ -360,16 +375,22 @@ template <typename E, bool TAIL, bool HARD> __global__ __launch_bounds__(64) voi
     }
     Elt<E>::st(dz + id, kept(id, q));
   }
-  if (hard && !bad_y && !__any(y_kept) && lane == 0 && mine(y)) {
+  if (!hard || bad_y) return;
+  __syncthreads();
+  if (!y_kept && tid == 0 && mine(y)) {
     Elt<E>::st(dz + y, grad(Elt<E>::ld(p + y)) - gh);
   }
 }
 
-// Segments per row: 32 waves per CU when every row is one wave; with fewer rows split, but no segment under four rounds of the wave's loads
-static void distill_split(int N, int V, int vec, int* S, int* seg_vecs) {
+// Waves and segments per row: one wave for short rows (under 16 KB there is nothing to share), four for long ones -- a row is then read by
+// one workgroup front to back, which the memory serves better than 4 x as many rows at once.  With few rows they are split, but no
+// segment gets under two rounds of the workgroup's loads.
+static void distill_split(int N, int V, int vec, int* W, int* S, int* seg_vecs) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
   const int nv = (V + vec - 1) / vec;
-  const int want = (16 * cus + N - 1) / N, most = (nv + 511) / 512;
+  *W = nv >= 1024 ? 4 : 1;
+  const int round = 64 * *W * (16 / vec);
+  const int want = (16 * cus / *W + N - 1) / N, most = (nv + 2 * round - 1) / (2 * round);
   int n = want < most ? want : most;
   const int least = (nv + 32767) / 32768;                     // (a segment's bitmap stays at 32 KB of LDS)
   if (n < least) n = least;
@@ -378,24 +399,29 @@ static void distill_split(int N, int V, int vec, int* S, int* seg_vecs) {
   *S = (nv + *seg_vecs - 1) / *seg_vecs;
 }
 
-template <typename E, bool TAIL> static int distill_fwd_launch(const DistillArgs& a, bool hard, int reduce, float* out, hipStream_t st) {
+template <typename E, bool TAIL, int W> static int distill_fwd_launch(const DistillArgs& a, bool hard, int reduce, float* out, hipStream_t st) {
   const unsigned ids = (unsigned)((a.K + 3) / 4 * 16);
   const unsigned bits = TAIL ? (unsigned)((a.seg_vecs * Elt<E>::kVec + 2 * Elt<E>::kVec + 31) / 32 * 4) : 0u;
   const dim3 grid((unsigned)a.N, (unsigned)a.S);
-  if (hard) VLN_LAUNCH((distill_fwd_kernel<E, TAIL, true>), grid, dim3(64), ids + bits, st, a);
-  else VLN_LAUNCH((distill_fwd_kernel<E, TAIL, false>), grid, dim3(64), ids + bits, st, a);
+  if (hard) VLN_LAUNCH((distill_fwd_kernel<E, TAIL, true, W>), grid, dim3(64 * W), ids + bits, st, a);
+  else VLN_LAUNCH((distill_fwd_kernel<E, TAIL, false, W>), grid, dim3(64 * W), ids + bits, st, a);
   if (a.S > 1) VLN_LAUNCH((distill_join_kernel<E, TAIL>), dim3((unsigned)a.N), dim3(64), ids, st, a);
   if (reduce) VLN_LAUNCH(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, (const float*)a.rows, (const float*)a.stats, a.N, reduce == VLN_REDUCE_MEAN ? 1 : 0, out);
   VLN_CHECK_LAUNCH("distill_fwd");
   return VLN_OK;
 }
-template <typename E, bool TAIL> static int distill_bwd_launch(const DistillArgs& a, bool hard, hipStream_t st) {
+template <typename E, bool TAIL, int W> static int distill_bwd_launch(const DistillArgs& a, bool hard, hipStream_t st) {
   const dim3 grid((unsigned)a.N, (unsigned)a.S);
   const unsigned ids = (unsigned)((a.K + 3) / 4 * 16);
-  if (hard) VLN_LAUNCH((distill_bwd_kernel<E, TAIL, true>), grid, dim3(64), ids, st, a);
-  else VLN_LAUNCH((distill_bwd_kernel<E, TAIL, false>), grid, dim3(64), ids, st, a);
+  if (hard) VLN_LAUNCH((distill_bwd_kernel<E, TAIL, true, W>), grid, dim3(64 * W), ids, st, a);
+  else VLN_LAUNCH((distill_bwd_kernel<E, TAIL, false, W>), grid, dim3(64 * W), ids, st, a);
   VLN_CHECK_LAUNCH("distill_bwd");
   return VLN_OK;
+}
+template <typename F> static int distill_dispatch(const DistillArgs& a, int type, F&& f) {      // f(element, with rest, waves)
+  auto waves = [&](auto e, auto tail) { return a.W == 4 ? f(e, tail, std::integral_constant<int, 4>()) : f(e, tail, std::integral_constant<int, 1>()); };
+  auto rest = [&](auto e) { return a.t_rest ? waves(e, std::true_type()) : waves(e, std::false_type()); };
+  return type == VLN_F32 ? rest(float()) : rest(bf16_raw());
 }
 
 static int distill_args(const vln_distill* p, DistillArgs& a, const char* who) {
@@ -421,7 +447,7 @@ static int distill_args(const vln_distill* p, DistillArgs& a, const char* who) {
   a.N = p->N; a.V = p->V; a.K = p->K;
   a.c = kLog2e / p->temperature; a.invT = 1.f / p->temperature; a.T = p->temperature; a.alpha = p->alpha;
   a.rows = p->rows; a.stats = p->stats;
-  distill_split(a.N, a.V, p->type == VLN_F32 ? 4 : 8, &a.S, &a.seg_vecs);
+  distill_split(a.N, a.V, p->type == VLN_F32 ? 4 : 8, &a.W, &a.S, &a.seg_vecs);
   return VLN_OK;
 }
 
@@ -429,8 +455,8 @@ static int distill_args(const vln_distill* p, DistillArgs& a, const char* who) {
 
 extern "C" int64_t vln_distill_ws_bytes(int N, int V, int type) {
   if (N <= 0 || V <= 0 || (type != VLN_F32 && type != VLN_BF16)) return 0;
-  int S, sv;
-  vln::distill_split(N, V, type == VLN_F32 ? 4 : 8, &S, &sv);
+  int W, S, sv;
+  vln::distill_split(N, V, type == VLN_F32 ? 4 : 8, &W, &S, &sv);
   return S > 1 ? (int64_t)N * S * 16 : 0;
 }
 extern "C" int vln_distill_fwd(const vln_distill* p, int reduction, float* out, void* ws, int64_t ws_bytes, vln_stream_t s) {
@@ -446,8 +472,9 @@ extern "C" int vln_distill_fwd(const vln_distill* p, int reduction, float* out, 
   }
   const bool hard = a.alpha < 1.f && a.T != 1.f;
   hipStream_t st = (hipStream_t)s;
-  if (p->type == VLN_F32) return a.t_rest ? vln::distill_fwd_launch<float, true>(a, hard, reduction, out, st) : vln::distill_fwd_launch<float, false>(a, hard, reduction, out, st);
-  return a.t_rest ? vln::distill_fwd_launch<bf16_raw, true>(a, hard, reduction, out, st) : vln::distill_fwd_launch<bf16_raw, false>(a, hard, reduction, out, st);
+  return vln::distill_dispatch(a, p->type, [&](auto e, auto tail, auto w) {
+    return vln::distill_fwd_launch<decltype(e), decltype(tail)::value, decltype(w)::value>(a, hard, reduction, out, st);
+  });
 }
 extern "C" int vln_distill_bwd(const vln_distill* p, const float* dloss, int64_t dloss_stride, const float* inv_count, void* dlogits, int64_t ld_dlogits,
                                vln_stream_t s) {
@@ -458,6 +485,7 @@ extern "C" int vln_distill_bwd(const vln_distill* p, const float* dloss, int64_t
   a.g = dloss; a.g_stride = (long)dloss_stride; a.inv_count = inv_count; a.dz = dlogits; a.ldz = ld_dlogits;
   const bool hard = a.alpha < 1.f && a.T != 1.f;
   hipStream_t st = (hipStream_t)s;
-  if (p->type == VLN_F32) return a.t_rest ? vln::distill_bwd_launch<float, true>(a, hard, st) : vln::distill_bwd_launch<float, false>(a, hard, st);
-  return a.t_rest ? vln::distill_bwd_launch<bf16_raw, true>(a, hard, st) : vln::distill_bwd_launch<bf16_raw, false>(a, hard, st);
+  return vln::distill_dispatch(a, p->type, [&](auto e, auto tail, auto w) {
+    return vln::distill_bwd_launch<decltype(e), decltype(tail)::value, decltype(w)::value>(a, hard, st);
+  });
 }
