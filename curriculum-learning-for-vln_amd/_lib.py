@@ -299,7 +299,7 @@ SIGNATURES = {
     "vln_top_logits_ws_bytes": (i64, [i32, i32, i32, i32]),
     "vln_top_logits": (i32, [ptr, i64, i32, i32, i32, i32, f32, ptr, ptr, ptr, ptr, i64, ptr]),
     "vln_distill_ws_bytes": (i64, [i32, i32, i32]),
-    "vln_distill_fwd": (i32, [C.POINTER(Distill), i32, ptr, ptr, i64, ptr]),
+    "vln_distill_fwd": (i32, [C.POINTER(Distill), i32, ptr, ptr, ptr, i64, ptr]),
     "vln_distill_bwd": (i32, [C.POINTER(Distill), ptr, i64, ptr, ptr, i64, ptr]),
     "vln_categorical_fwd": (i32, [ptr, i64, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, u64, u64, ptr, ptr]),
     "vln_categorical_bwd": (i32, [ptr, ptr, ptr, ptr, ptr, i32, i32, ptr]),

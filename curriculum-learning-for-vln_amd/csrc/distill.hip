@@ -16,7 +16,7 @@
 namespace vln {
 
 constexpr int kStat = VLN_DISTILL_STATS;      // per row: see the enum
-enum { ST_FLAGS = 0, ST_M, ST_S, ST_S1, ST_MR, ST_SR, ST_TM, ST_TS, ST_R };
+enum { ST_FLAGS = 0, ST_M, ST_S, ST_S1, ST_MR, ST_SR, ST_TM, ST_TS, ST_R };      // (finish_row writes them in this order)
 enum { ROW_LIVE = 1, ROW_SOFT = 2, ROW_TWICE = 4 };      // counted; the teacher has mass; some kept word is listed twice
 
 struct DistillArgs {
@@ -31,6 +31,7 @@ struct DistillArgs {
   float* rows; float* stats;
   float4* part;               // S > 1: [N, S]
   // backward
+  int stream;                 // the gradient is larger than the caches: it is written past them
   void* dz; int64_t ldz; const float* g; long g_stride; const float* inv_count;
 };
 
@@ -45,51 +46,77 @@ __device__ __forceinline__ float teacher_u(const DistillArgs& a, long n, int j) 
 }
 __device__ __forceinline__ bool row_ignored(const DistillArgs& a, long n) { return a.target && (long)a.target[n] == a.ignore; }
 
+// The kept words of a row in registers, entry j of thread j % B: ids are asked for first, the student's logits at them as soon as they
+// are there, so that neither waits behind the stream of the row.
+template <int B> struct Kept {
+  static constexpr int R = VLN_DISTILL_MAX / B;
+  int id[R];             // -1: absent
+  float u[R], z[R];      // t / T, the student's logit
+  __device__ __forceinline__ void ask(const DistillArgs& a, long n, int tid) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      id[i] = -1;
+      u[i] = z[i] = 0.f;
+      const int j = i * B + tid;
+      if (j < a.K) {
+        const long long v = a.ids[n * a.ld_ids + j];
+        id[i] = v >= 0 && v < a.V ? (int)v : -1;
+        u[i] = teacher_u(a, n, j);
+      }
+    }
+  }
+  template <typename E> __device__ __forceinline__ void gather(const E* p) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) if (id[i] >= 0) z[i] = Elt<E>::ld(p + id[i]);
+  }
+  template <typename F> __device__ __forceinline__ void each(F&& f) const {      // f(i): the entries present
+#pragma unroll
+    for (int i = 0; i < R; ++i) if (id[i] >= 0) f(i);
+  }
+};
+
 // Everything of a row that does not need the whole row again, by one wave.  dense / s1: the (maximum, sum) over all words -- or, TAIL,
-// over the words outside `kid` -- at temperature T, and the sum at temperature 1 relative to the same maximum (hard targets).
-// kid [K]: the row's word ids in LDS (-1: absent).
-template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(const DistillArgs& a, long n, OnlineSum dense, float s1, const int* kid,
-                                                                            int lane) {
-  const E* p = static_cast<const E*>(a.logits) + n * a.ld;
+// over the words that are not kept -- at temperature T, and the sum at temperature 1 relative to the same maximum (hard targets).
+// kid [K]: the row's word ids in LDS (-1: absent); twice: some word may be listed twice; zy: the student's logit at the target.
+template <bool TAIL> __device__ __forceinline__ void finish_row(const DistillArgs& a, long n, const Kept<64>& k, OnlineSum dense, float s1,
+                                                                const int* kid, bool twice, float rest, float zy, int lane) {
   const float c = a.c;
   // teacher: maximum and sum over the outcomes present
   float tm = -INFINITY;
   bool nan = false;                  // (no maximum takes a NaN: it enters through the sum, and the row's loss is NaN)
   auto outcome = [&](float u) { tm = fmaxf(tm, u); nan = nan || u != u; };
-  if (TAIL) outcome(a.t_rest[n]);
-  for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) outcome(teacher_u(a, n, j));
+  if (TAIL) outcome(rest);
+  k.each([&](int i) { outcome(k.u[i]); });
   tm = wave_fmax(tm);
   const bool soft = tm != -INFINITY || __any(nan);
   const float tref = tm != -INFINITY ? tm : 0.f;
   float ts = 0.f;
-  for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) ts += exp2_hw((teacher_u(a, n, j) - tref) * kLog2e);
-  ts = wave_fsum(ts);
-  const float er = TAIL ? exp2_hw((a.t_rest[n] - tref) * kLog2e) : 0.f;
-  ts += er;
+  k.each([&](int i) { ts += exp2_hw((k.u[i] - tref) * kLog2e); });
+  const float er = TAIL ? exp2_hw((rest - tref) * kLog2e) : 0.f;
+  ts = wave_fsum(ts) + er;
   // a word listed twice: only its first entry counts in the student's total
-  bool twice = false;
-  for (int j = lane; j < a.K; j += 64) {
-    const int id = kid[j];
-    if (id >= 0) for (int i = 0; i < j; ++i) twice = twice || kid[i] == id;
+  bool again[Kept<64>::R] = {};
+  if (twice) {
+    twice = false;
+    k.each([&](int i) {
+      for (int j = 0; j < i * 64 + lane; ++j) again[i] = again[i] || kid[j] == k.id[i];
+      twice = twice || again[i];
+    });
+    twice = __any(twice);
   }
-  const bool any_twice = __any(twice);
   // student
   OnlineSum all = dense;
   if (TAIL) {
     float M = dense.m;
-    for (int j = lane; j < a.K; j += 64) if (kid[j] >= 0) M = fmaxf(M, Elt<E>::ld(p + kid[j]));
+    k.each([&](int i) { M = fmaxf(M, k.z[i]); });
     M = wave_fmax(M);
     float t = 0.f, t1 = 0.f;
-    for (int j = lane; j < a.K; j += 64) {
-      const int id = kid[j];
-      bool first = id >= 0;
-      if (any_twice) for (int i = 0; i < j; ++i) first = first && kid[i] != id;
-      if (first) {
-        const float d = Elt<E>::ld(p + id) - M;
-        t += exp2_hw(d * c);
-        t1 += exp2_hw(d * kLog2e);
-      }
-    }
+    k.each([&](int i) {
+      if (again[i]) return;
+      const float d = k.z[i] - M;
+      t += exp2_hw(d * c);
+      t1 += exp2_hw(d * kLog2e);
+    });
     all.s = dense.s * exp2_hw((dense.m - M) * c) + wave_fsum(t);
     s1 = s1 * exp2_hw((dense.m - M) * kLog2e) + wave_fsum(t1);
     all.m = M;
@@ -97,40 +124,36 @@ template <typename E, bool TAIL> __device__ __forceinline__ void finish_row(cons
   const float log_s = logf(all.s), log_ts = logf(ts);
   float loss = 0.f;
   if (soft) {
-    for (int j = lane; j < a.K; j += 64) {
-      const int id = kid[j];
-      if (id < 0) continue;
-      const float lq = (teacher_u(a, n, j) - tref) - log_ts, q = exp2_hw(lq * kLog2e);
-      const float z = Elt<E>::ld(p + id);
-      const float lp = z == -INFINITY ? -INFINITY : (z - all.m) * a.invT - log_s;
+    k.each([&](int i) {
+      const float lq = (k.u[i] - tref) - log_ts, q = exp2_hw(lq * kLog2e);
+      const float lp = k.z[i] == -INFINITY ? -INFINITY : (k.z[i] - all.m) * a.invT - log_s;
       if (q != 0.f) loss += q * (lq - lp);
-    }
+    });
     if (TAIL && lane == 0 && er != 0.f) {
-      const float lr = (a.t_rest[n] - tref) - log_ts;
+      const float lr = (rest - tref) - log_ts;
       const float lpr = dense.s == 0.f ? -INFINITY : (dense.m - all.m) * a.invT + logf(dense.s) - log_s;
       loss += exp2_hw(lr * kLog2e) * (lr - lpr);
     }
   }
   loss = wave_fsum(loss) * a.alpha * a.T * a.T;
   if (a.alpha == 0.f) loss = 0.f;
-  const bool live = a.target ? !row_ignored(a, n) : soft;
-  if (a.target && a.alpha < 1.f) {
-    const long y = (long)a.target[n];
-    const float z = (y >= 0 && y < a.V) ? Elt<E>::ld(p + y) : __builtin_nanf("");
-    loss += (1.f - a.alpha) * (all.m - z + logf(s1));
-  }
+  const bool live = a.target ? true : soft;          // (ignored rows do not come here)
+  if (a.target && a.alpha < 1.f) loss += (1.f - a.alpha) * (all.m - zy + logf(s1));
   if (lane == 0) {
     a.rows[n] = live ? loss : 0.f;
-    float* st = a.stats + n * kStat;
-    st[ST_FLAGS] = __int_as_float((live ? ROW_LIVE : 0) | (soft ? ROW_SOFT : 0) | (any_twice ? ROW_TWICE : 0));
-    st[ST_M] = all.m; st[ST_S] = all.s; st[ST_S1] = s1;
-    st[ST_MR] = dense.m; st[ST_SR] = dense.s;
-    st[ST_TM] = tref; st[ST_TS] = ts;
-    st[ST_R] = soft ? er / ts : 0.f;
+    float4* st = reinterpret_cast<float4*>(a.stats + n * kStat);
+    st[0] = make_float4(__int_as_float((live ? ROW_LIVE : 0) | (soft ? ROW_SOFT : 0) | (twice ? ROW_TWICE : 0)), all.m, all.s, s1);
+    st[1] = make_float4(dense.m, dense.s, tref, ts);
+    st[2] = make_float4(soft ? er / ts : 0.f, 0.f, 0.f, 0.f);
   }
 }
+template <typename E> __device__ __forceinline__ float target_logit(const DistillArgs& a, long n, const E* p) {      // NaN: no such word
+  if (!a.target || a.alpha >= 1.f) return 0.f;
+  const long y = (long)a.target[n];
+  return y >= 0 && y < a.V ? Elt<E>::ld(p + y) : __builtin_nanf("");
+}
 __device__ __forceinline__ void dead_row(const DistillArgs& a, long n, int lane) {
-  if (lane == 0) { a.rows[n] = 0.f; a.stats[n * kStat + ST_FLAGS] = __int_as_float(0); }
+  if (lane == 0) { a.rows[n] = 0.f; a.stats[n * kStat] = __int_as_float(0); }
 }
 // one wave joins the (maximum, sum at T, sum at 1) of `count` parts, in their order per lane
 __device__ __forceinline__ void join_parts(OnlineSum& o, float& s1, const float4* parts, int count, float c, int lane) {
@@ -146,41 +169,67 @@ __device__ __forceinline__ void join_parts(OnlineSum& o, float& s1, const float4
   s1 = wave_fsum(s1 * exp2_hw((o.m - M) * kLog2e));
   o.wave(c);
 }
-template <int B> __device__ __forceinline__ void stage_ids(const DistillArgs& a, long n, int* kid, int tid) {
-  for (int j = tid; j < a.K; j += B) {
-    const long long id = a.ids[n * a.ld_ids + j];
-    kid[j] = (id >= 0 && id < a.V) ? (int)id : -1;
+// kid <- the ids; true if two of the wave's entries may name the same word: their bits in a table of 2^14 meet (then the list is searched)
+constexpr int kHashWords = 512;
+__device__ __forceinline__ bool stage_ids(const DistillArgs& a, const Kept<64>& k, int* kid, unsigned* hash, int lane) {
+  for (int i = lane; i < kHashWords; i += 64) hash[i] = 0u;
+  wave_sync();
+  bool met = false;
+#pragma unroll
+  for (int i = 0; i < Kept<64>::R; ++i) {
+    if (i * 64 + lane < a.K) kid[i * 64 + lane] = k.id[i];
+    if (k.id[i] >= 0) {
+      const unsigned h = (unsigned)k.id[i] & (kHashWords * 32 - 1);
+      met = met || ((atomicOr(&hash[h >> 5], 1u << (h & 31)) >> (h & 31)) & 1u);
+    }
   }
-  __syncthreads();
+  wave_sync();
+  return __any(met);
 }
 
 // HARD: also the sum at temperature 1 (T != 1 and a hard target); otherwise s1 is the sum at T.  W: waves of a row (or segment).
 template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(64 * W) void distill_fwd_kernel(DistillArgs a) {
   extern __shared__ unsigned lds[];
-  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC, B = 64 * W;
+  constexpr int VEC = RowGeo<E>::VEC, U = 4, B = 64 * W;
   const long n = blockIdx.x;
   const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   if (row_ignored(a, n)) { if (s == 0) dead_row(a, n, tid); return; }
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   const RowGeo<E> g(p, a.V);
   const int v0 = min(g.nv, s * a.seg_vecs), v1 = min(g.nv, v0 + a.seg_vecs);
+  const bool finishes = a.S == 1 && w == 0;
+  Kept<64> k;
+  if (finishes || (TAIL && w == 0)) k.ask(a, n, lane);
+  float rest = 0.f, zy = 0.f;
+  if (finishes) { rest = TAIL ? a.t_rest[n] : 0.f; zy = target_logit(a, n, p); }
+  uint4 raw[U];
+  auto fetch = [&](int v) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * B, v1 - 1) * VEC);
+  };
+  if (v0 + tid < v1) fetch(v0 + tid);
   int* kid = reinterpret_cast<int*>(lds);
-  unsigned* bm = lds + (a.K + 3) / 4 * 4;        // bit i: column i of the segment's vectors; then head, then tail (VEC bits each)
+  unsigned* bm = lds + VLN_DISTILL_MAX + kHashWords;       // bit i: column i of the segment's vectors; then head, then tail (VEC bits each)
   const int nbits_v = a.seg_vecs * VEC;
-  if (TAIL || a.S == 1) stage_ids<B>(a, n, kid, tid);
+  bool twice = false;
   if (TAIL) {
     const int nw = (nbits_v + 2 * VEC + 31) / 32;
     for (int i = tid; i < nw; i += B) bm[i] = 0u;
     __syncthreads();
-    for (int j = tid; j < a.K; j += B) {
-      const int id = kid[j];
-      if (id < 0) continue;
+  }
+  if (finishes) {
+    twice = stage_ids(a, k, kid, lds + VLN_DISTILL_MAX, lane);
+    k.gather(p);
+  }
+  if (TAIL) {
+    if (w == 0) k.each([&](int i) {
+      const int id = k.id[i];
       int bit = -1;
       if (id < g.head) bit = nbits_v + id;
       else if (id >= g.tail0()) bit = nbits_v + VEC + (id - g.tail0());
-      else { const int i = id - g.head - v0 * VEC; if (i >= 0 && i < (v1 - v0) * VEC) bit = i; }
+      else { const int at = id - g.head - v0 * VEC; if (at >= 0 && at < (v1 - v0) * VEC) bit = at; }
       if (bit >= 0) atomicOr(&bm[bit >> 5], 1u << (bit & 31));
-    }
+    });
     __syncthreads();
   }
   OnlineSum o;
@@ -210,10 +259,7 @@ template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(
     take(x, x[0]);
   }
   for (int v = v0 + tid; v < v1; v += B * U) {
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * B, v1 - 1) * VEC);
-    float x[16];
+    float x[U * VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       unpack16<E>(raw[u], x + u * VEC);
@@ -225,9 +271,10 @@ template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(
         for (int j = 0; j < VEC; ++j) if ((out >> j) & 1u) x[u * VEC + j] = -INFINITY;
       }
     }
+    if (v + B * U < v1) fetch(v + B * U);
     float mx = x[0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) mx = fmaxf(mx, x[j]);
+    for (int j = 1; j < U * VEC; ++j) mx = fmaxf(mx, x[j]);
     take(x, mx);
   }
   const float M = wave_fmax(o.m);
@@ -242,25 +289,31 @@ template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(
     if (w > 0) return;
     join_parts(o, s1, parts, W, a.c, lane);
   }
-  if (a.S == 1) finish_row<E, TAIL>(a, n, o, s1, kid, lane);
+  if (finishes) finish_row<TAIL>(a, n, k, o, s1, kid, twice, rest, zy, lane);
   else if (lane == 0) a.part[n * a.S + s] = make_float4(o.m, o.s, s1, 0.f);
 }
 
 template <typename E, bool TAIL> __global__ __launch_bounds__(64) void distill_join_kernel(DistillArgs a) {
-  extern __shared__ unsigned lds[];
+  __shared__ int kid[VLN_DISTILL_MAX];
+  __shared__ unsigned hash[kHashWords];
   const long n = blockIdx.x;
   const int lane = threadIdx.x;
   if (row_ignored(a, n)) return;
-  int* kid = reinterpret_cast<int*>(lds);
-  stage_ids<64>(a, n, kid, lane);
+  const E* p = static_cast<const E*>(a.logits) + n * a.ld;
+  Kept<64> k;
+  k.ask(a, n, lane);
+  const float rest = TAIL ? a.t_rest[n] : 0.f, zy = target_logit(a, n, p);
   OnlineSum o;
   float s1;
   join_parts(o, s1, a.part + n * a.S, a.S, a.c, lane);
-  finish_row<E, TAIL>(a, n, o, s1, kid, lane);
+  const bool twice = stage_ids(a, k, kid, hash, lane);
+  k.gather(p);
+  __syncthreads();
+  finish_row<TAIL>(a, n, k, o, s1, kid, twice, rest, zy, lane);
 }
 
-// sum or mean over the rows, in a fixed order: out[0] = loss, out[1] = what the backward multiplies every row's gradient with
-__global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows, const float* stats, int N, int mean, float* out) {
+// sum or mean over the rows, in a fixed order; inv_count: what the backward multiplies every row's gradient with
+__global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows, const float* stats, int N, int mean, float* loss, float* inv_count) {
   __shared__ float part[16];
   __shared__ int cnt[16];
   float acc = 0.f;
@@ -278,8 +331,8 @@ __global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows,
     float t = 0.f;
     int c = 0;
     for (int i = 0; i < 16; ++i) { t += part[i]; c += cnt[i]; }
-    out[0] = mean ? t / (float)c : t;
-    out[1] = mean ? 1.f / (float)c : 1.f;
+    loss[0] = mean ? t / (float)c : t;
+    inv_count[0] = mean ? 1.f / (float)c : 1.f;
   }
 }
 
@@ -288,13 +341,15 @@ __global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* rows,
 // that loop are bounded by (TAIL: the others' maximum), so neither a sure student's tiny p_rest nor its kept words leave the range.
 template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(64 * W) void distill_bwd_kernel(DistillArgs a) {
   extern __shared__ unsigned lds[];
-  constexpr int VEC = RowGeo<E>::VEC, U = 16 / VEC, B = 64 * W;
+  constexpr int VEC = RowGeo<E>::VEC, U = 4, B = 64 * W;
   __shared__ int y_kept;
-  const long n = blockIdx.x;
+  const long n = gridDim.x - 1 - blockIdx.x;         // the rows the forward read last come first: the caches still hold them
   const int s = blockIdx.y, tid = threadIdx.x;
   if (tid == 0) y_kept = 0;
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   E* dz = static_cast<E*>(a.dz) + n * a.ldz;
+  Kept<B> k;
+  k.ask(a, n, tid);
   const float* st = a.stats + n * kStat;
   const int flags = __float_as_int(st[ST_FLAGS]);
   const RowGeo<E> g(dz, a.V);                 // the writes decide the alignment
@@ -302,15 +357,32 @@ template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(
   const int v0 = min(g.nv, s * a.seg_vecs), v1 = min(g.nv, v0 + a.seg_vecs);
   const bool single = s == 0 && (tid < g.head || (tid >= VEC && tid - VEC < g.tail));
   const int scol = tid < g.head ? tid : g.tail0() + tid - VEC;
+  auto put = [&](E* at, const uint4& v) { if (a.stream) st_vec_nt<E>(at, v); else st_vec<E>(at, v); };
   if (!(flags & ROW_LIVE)) {                  // an ignored row: zeros, whatever its logits hold
     if (single) Elt<E>::st(dz + scol, 0.f);
-    for (int v = v0 + tid; v < v1; v += B) st_vec<E>(dz + g.head + (int64_t)v * VEC, make_uint4(0, 0, 0, 0));
+    for (int v = v0 + tid; v < v1; v += B) put(dz + g.head + (int64_t)v * VEC, make_uint4(0, 0, 0, 0));
     return;
+  }
+  uint4 raw[U];
+  auto fetch = [&](int v) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * B, v1 - 1) * VEC);
+  };
+  if (same && v0 + tid < v1) fetch(v0 + tid);
+  auto here = [&](int id) {                   // a column of this segment
+    if (id < g.head || id >= g.tail0()) return s == 0;
+    const int i = (id - g.head) / VEC;
+    return i >= v0 && i < v1;
+  };
+  int* kid = reinterpret_cast<int*>(lds);
+  if (flags & ROW_TWICE) {
+#pragma unroll
+    for (int i = 0; i < Kept<B>::R; ++i) if (i * B + tid < a.K) kid[i * B + tid] = k.id[i];
   }
   const float up = a.g[n * a.g_stride] * (a.inv_count ? a.inv_count[0] : 1.f);
   const bool soft = (flags & ROW_SOFT) != 0 && a.alpha != 0.f;
   const float m = st[ST_M], sum = st[ST_S], s1 = st[ST_S1], r = TAIL ? st[ST_R] : 0.f;
-  const float M = TAIL ? st[ST_MR] : m, sr = st[ST_SR];
+  const float M = TAIL ? st[ST_MR] : m, sr = st[ST_SR], tm = st[ST_TM], its = 1.f / st[ST_TS];
   const float gs = soft ? up * a.alpha * a.T : 0.f;                  // soft term's factor
   const bool hard = a.target != nullptr && a.alpha < 1.f;
   const float gh = hard ? up * (1.f - a.alpha) : 0.f;
@@ -327,59 +399,46 @@ template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(
     if (HARD) v += H * exp2_hw(d * kLog2e);
     return v;
   };
+  // (kept words matter if they have a share of the gradient, or if the streaming loop's factors are not theirs)
+  if (soft || TAIL) {
+    k.gather(p);
+    k.each([&](int i) { if (k.id[i] == y) y_kept = 1; });
+  }
   if (single) Elt<E>::st(dz + scol, grad(Elt<E>::ld(p + scol)));
   if (same) {
     for (int v = v0 + tid; v < v1; v += B * U) {
-      uint4 raw[U];
+      uint4 now[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = ld_vec<E>(p + g.head + (int64_t)min(v + u * B, v1 - 1) * VEC);
+      for (int u = 0; u < U; ++u) now[u] = raw[u];
+      if (v + B * U < v1) fetch(v + B * U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float x[VEC];
-        unpack16<E>(raw[u], x);
+        unpack16<E>(now[u], x);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) x[j] = grad(x[j]);
-        if (v + u * B < v1) st_vec<E>(dz + g.head + (int64_t)(v + u * B) * VEC, pack16<E>(x));
+        if (v + u * B < v1) put(dz + g.head + (int64_t)(v + u * B) * VEC, pack16<E>(x));
       }
     }
   } else {                                    // rows that start at different distances from a 16-byte boundary
     for (int c = g.head + v0 * VEC + tid; c < g.head + v1 * VEC; c += B) Elt<E>::st(dz + c, grad(Elt<E>::ld(p + c)));
   }
   // the kept words and the target: their own values over what the loop wrote
-  int* kid = reinterpret_cast<int*>(lds);
-  const int nk = soft || TAIL ? a.K : 0;
-  if (nk) stage_ids<B>(a, n, kid, tid); else __syncthreads();
-  auto mine = [&](long id) {
-    if (id < g.head || id >= g.tail0()) return s == 0;
-    const int i = (int)((id - g.head) / VEC);
-    return i >= v0 && i < v1;
-  };
-  const float tm = st[ST_TM], its = 1.f / st[ST_TS];
-  auto kept = [&](int id, float q) {          // gradient of a word with the teacher's probability q
-    const float d = Elt<E>::ld(p + id) - m;
+  __syncthreads();
+  if (soft || TAIL) k.each([&](int i) {
+    const int id = k.id[i], j = i * B + tid;
+    if (!here(id)) return;
+    float q = soft ? exp2_hw((k.u[i] - tm) * kLog2e) * its : 0.f;
+    if (soft && (flags & ROW_TWICE)) {        // listed more than once: the first entry writes the sum, in entry order
+      for (int e = 0; e < j; ++e) if (kid[e] == id) return;
+      for (int e = j + 1; e < a.K; ++e) if (kid[e] == id) q += exp2_hw((teacher_u(a, n, e) - tm) * kLog2e) * its;
+    }
+    const float d = k.z[i] - m;
     float v = gs * (exp2_hw(d * a.c) * is - q);
     if (hard) v += gh * (exp2_hw(d * kLog2e) * is1 - (id == y ? 1.f : 0.f));
-    return bad_y ? __builtin_nanf("") : v;
-  };
-  for (int j = tid; j < nk; j += B) {
-    const int id = kid[j];
-    if (id < 0) continue;
-    if (id == y) y_kept = 1;
-    if (!mine(id)) continue;
-    float q = soft ? exp2_hw((teacher_u(a, n, j) - tm) * kLog2e) * its : 0.f;
-    if (soft && (flags & ROW_TWICE)) {                  // listed more than once: the first entry writes the sum, in entry order
-      bool first = true;
-      for (int i = 0; i < j; ++i) first = first && kid[i] != id;
-      if (!first) continue;
-      for (int i = j + 1; i < a.K; ++i) if (kid[i] == id) q += exp2_hw((teacher_u(a, n, i) - tm) * kLog2e) * its;
-    }
-    Elt<E>::st(dz + id, kept(id, q));
-  }
-  if (!hard || bad_y) return;
-  __syncthreads();
-  if (!y_kept && tid == 0 && mine(y)) {
-    Elt<E>::st(dz + y, grad(Elt<E>::ld(p + y)) - gh);
-  }
+    Elt<E>::st(dz + id, bad_y ? __builtin_nanf("") : v);
+  });
+  if (hard && !bad_y && !y_kept && tid == 0 && here((int)y)) Elt<E>::st(dz + y, grad(Elt<E>::ld(p + y)) - gh);
 }
 
 // Waves and segments per row: one wave for short rows (under 16 KB there is nothing to share), four for long ones -- a row is then read by
@@ -389,7 +448,7 @@ static void distill_split(int N, int V, int vec, int* W, int* S, int* seg_vecs) 
   const int cus = device_cus() > 0 ? device_cus() : 256;
   const int nv = (V + vec - 1) / vec;
   *W = nv >= 1024 ? 4 : 1;
-  const int round = 64 * *W * (16 / vec);
+  const int round = 64 * *W * 4;
   const int want = (16 * cus / *W + N - 1) / N, most = (nv + 2 * round - 1) / (2 * round);
   int n = want < most ? want : most;
   const int least = (nv + 32767) / 32768;                     // (a segment's bitmap stays at 32 KB of LDS)
@@ -399,20 +458,20 @@ static void distill_split(int N, int V, int vec, int* W, int* S, int* seg_vecs) 
   *S = (nv + *seg_vecs - 1) / *seg_vecs;
 }
 
-template <typename E, bool TAIL, int W> static int distill_fwd_launch(const DistillArgs& a, bool hard, int reduce, float* out, hipStream_t st) {
-  const unsigned ids = (unsigned)((a.K + 3) / 4 * 16);
+template <typename E, bool TAIL, int W> static int distill_fwd_launch(const DistillArgs& a, bool hard, int reduce, float* loss, float* inv_count, hipStream_t st) {
+  const unsigned ids = (VLN_DISTILL_MAX + kHashWords) * 4;
   const unsigned bits = TAIL ? (unsigned)((a.seg_vecs * Elt<E>::kVec + 2 * Elt<E>::kVec + 31) / 32 * 4) : 0u;
   const dim3 grid((unsigned)a.N, (unsigned)a.S);
   if (hard) VLN_LAUNCH((distill_fwd_kernel<E, TAIL, true, W>), grid, dim3(64 * W), ids + bits, st, a);
   else VLN_LAUNCH((distill_fwd_kernel<E, TAIL, false, W>), grid, dim3(64 * W), ids + bits, st, a);
-  if (a.S > 1) VLN_LAUNCH((distill_join_kernel<E, TAIL>), dim3((unsigned)a.N), dim3(64), ids, st, a);
-  if (reduce) VLN_LAUNCH(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, (const float*)a.rows, (const float*)a.stats, a.N, reduce == VLN_REDUCE_MEAN ? 1 : 0, out);
+  if (a.S > 1) VLN_LAUNCH((distill_join_kernel<E, TAIL>), dim3((unsigned)a.N), dim3(64), 0, st, a);
+  if (reduce) VLN_LAUNCH(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, (const float*)a.rows, (const float*)a.stats, a.N, reduce == VLN_REDUCE_MEAN ? 1 : 0, loss, inv_count);
   VLN_CHECK_LAUNCH("distill_fwd");
   return VLN_OK;
 }
 template <typename E, bool TAIL, int W> static int distill_bwd_launch(const DistillArgs& a, bool hard, hipStream_t st) {
   const dim3 grid((unsigned)a.N, (unsigned)a.S);
-  const unsigned ids = (unsigned)((a.K + 3) / 4 * 16);
+  const unsigned ids = VLN_DISTILL_MAX * 4;
   if (hard) VLN_LAUNCH((distill_bwd_kernel<E, TAIL, true, W>), grid, dim3(64 * W), ids, st, a);
   else VLN_LAUNCH((distill_bwd_kernel<E, TAIL, false, W>), grid, dim3(64 * W), ids, st, a);
   VLN_CHECK_LAUNCH("distill_bwd");
@@ -424,7 +483,7 @@ template <typename F> static int distill_dispatch(const DistillArgs& a, int type
   return type == VLN_F32 ? rest(float()) : rest(bf16_raw());
 }
 
-static int distill_args(const vln_distill* p, DistillArgs& a, const char* who) {
+static int distill_args(const vln_distill* p, DistillArgs& a, const char* who, bool backward) {
   if (!p) { set_error("%s: null pointer", who); return VLN_ERR_ARG; }
   if (p->N <= 0 || p->V <= 0 || !p->logits || p->ld < p->V) { set_error("%s: bad logits", who); return VLN_ERR_ARG; }
   if (p->K < 1 || p->K > VLN_DISTILL_MAX || !p->ids || !p->teacher || p->ld_ids < p->K || p->ld_teacher < p->K) {
@@ -437,7 +496,7 @@ static int distill_args(const vln_distill* p, DistillArgs& a, const char* who) {
     set_error("%s: bad temperature / alpha", who); return VLN_ERR_ARG;
   }
   if (p->alpha < 1.f && !p->target) { set_error("%s: alpha < 1 needs hard targets", who); return VLN_ERR_ARG; }
-  if (!p->rows || !p->stats) { set_error("%s: rows / stats missing", who); return VLN_ERR_ARG; }
+  if ((!p->rows && !backward) || !p->stats) { set_error("%s: rows / stats missing", who); return VLN_ERR_ARG; }
   a = DistillArgs{};
   a.logits = p->logits; a.ld = p->ld;
   a.ids = (const long long*)p->ids; a.ld_ids = p->ld_ids;
@@ -459,11 +518,11 @@ extern "C" int64_t vln_distill_ws_bytes(int N, int V, int type) {
   vln::distill_split(N, V, type == VLN_F32 ? 4 : 8, &W, &S, &sv);
   return S > 1 ? (int64_t)N * S * 16 : 0;
 }
-extern "C" int vln_distill_fwd(const vln_distill* p, int reduction, float* out, void* ws, int64_t ws_bytes, vln_stream_t s) {
+extern "C" int vln_distill_fwd(const vln_distill* p, int reduction, float* loss, float* inv_count, void* ws, int64_t ws_bytes, vln_stream_t s) {
   vln::DistillArgs a;
-  const int rc = vln::distill_args(p, a, "vln_distill_fwd");
+  const int rc = vln::distill_args(p, a, "vln_distill_fwd", false);
   if (rc != VLN_OK) return rc;
-  if ((reduction != VLN_REDUCE_NONE && reduction != VLN_REDUCE_SUM && reduction != VLN_REDUCE_MEAN) || (reduction != VLN_REDUCE_NONE && !out)) {
+  if ((reduction != VLN_REDUCE_NONE && reduction != VLN_REDUCE_SUM && reduction != VLN_REDUCE_MEAN) || (reduction != VLN_REDUCE_NONE && (!loss || !inv_count))) {
     vln::set_error("vln_distill_fwd: bad reduction"); return VLN_ERR_ARG;
   }
   if (a.S > 1) {
@@ -473,16 +532,18 @@ extern "C" int vln_distill_fwd(const vln_distill* p, int reduction, float* out, 
   const bool hard = a.alpha < 1.f && a.T != 1.f;
   hipStream_t st = (hipStream_t)s;
   return vln::distill_dispatch(a, p->type, [&](auto e, auto tail, auto w) {
-    return vln::distill_fwd_launch<decltype(e), decltype(tail)::value, decltype(w)::value>(a, hard, reduction, out, st);
+    return vln::distill_fwd_launch<decltype(e), decltype(tail)::value, decltype(w)::value>(a, hard, reduction, loss, inv_count, st);
   });
 }
 extern "C" int vln_distill_bwd(const vln_distill* p, const float* dloss, int64_t dloss_stride, const float* inv_count, void* dlogits, int64_t ld_dlogits,
                                vln_stream_t s) {
   vln::DistillArgs a;
-  const int rc = vln::distill_args(p, a, "vln_distill_bwd");
+  const int rc = vln::distill_args(p, a, "vln_distill_bwd", true);
   if (rc != VLN_OK) return rc;
   if (!dloss || (dloss_stride != 0 && dloss_stride != 1) || !dlogits || ld_dlogits < p->V) { vln::set_error("vln_distill_bwd: bad args"); return VLN_ERR_ARG; }
   a.g = dloss; a.g_stride = (long)dloss_stride; a.inv_count = inv_count; a.dz = dlogits; a.ldz = ld_dlogits;
+  // 8 dies x 4 MB of L2 cannot hold it (4096 x 32000 bf16: 202 -> 178 us)
+  a.stream = (int64_t)a.N * a.V * (p->type == VLN_F32 ? 4 : 2) > (32 << 20);
   const bool hard = a.alpha < 1.f && a.T != 1.f;
   hipStream_t st = (hipStream_t)s;
   return vln::distill_dispatch(a, p->type, [&](auto e, auto tail, auto w) {

@@ -42,6 +42,10 @@ template <> __device__ __forceinline__ uint4 pack16<bf16_raw>(const float* o) {
 template <typename E> __device__ __forceinline__ uint4 ld_vec(const E* p) { return *reinterpret_cast<const uint4*>(p); }
 template <typename E> __device__ __forceinline__ void st_vec(E* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
 
+template <typename E> __device__ __forceinline__ void st_vec_nt(E* p, const uint4& v) {
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), reinterpret_cast<u32x4_t*>(p));
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, results below 2^-126 are 0
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -113,6 +117,13 @@ struct OnlineSum {
     m = M;
   }
 };
+
+// what the wave's lanes wrote to LDS, visible to all of them (one wave's accesses are carried out in order; a workgroup barrier is not needed)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 __device__ __forceinline__ int lanes_below(unsigned long long mask) {
   return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));

@@ -8,30 +8,41 @@ fp32 or bf16 logits, rows any distance apart; arithmetic in fp32, one rounding t
 fallback.  Everything is launched on the current stream of the logits' device; nothing synchronises, nothing is kept between calls."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 from typing import Optional, Union
 
 import torch
 
 from . import _lib, losses, ops
 
-_p = ops._p
 _TYPES = {torch.float32: ops.F32, torch.bfloat16: ops.BF16}
+_byref = C.byref
 
 
-def _on(device):
-    """The launches go to the logits' device, also when another one is current."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(fn, name: str, device, *args):
+    """fn(*args, stream) on the current stream of the logits' device, also when another device is current."""
+    if device.index == _lib._get_device():
+        st = fn(*args, _lib.raw_stream())
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _lib.raw_stream())
+    if st:
+        _lib.check(st, name)
 
 
 def _rows(t: torch.Tensor, name: str):
-    """[N, V] word logits of a supported type, as rows of contiguous elements."""
+    """(N, V, type code) of word logits [N, V]."""
     losses._not_deferred(t, name)
-    if t.dtype not in _TYPES:
+    code = _TYPES.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name}: expected float32 or bfloat16 logits, got {t.dtype}")
-    if t.dim() != 2 or t.shape[1] < 1 or t.shape[0] >= 1 << 31 or t.shape[1] >= 1 << 31:
-        raise ValueError(f"{name}: expected logits [N, V] with V >= 1, got {tuple(t.shape)}")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected logits [N, V], got {tuple(t.shape)}")
+    N, V = t.shape
+    if V < 1 or N >= 1 << 31 or V >= 1 << 31:
+        raise ValueError(f"{name}: expected logits [N, V] with 1 <= V < 2^31, got {tuple(t.shape)}")
+    return N, V, code
 
 
 def _gpu(t: torch.Tensor, name: str):
@@ -39,13 +50,10 @@ def _gpu(t: torch.Tensor, name: str):
         raise _lib.VlnError(f"{name}: expected GPU tensors (the HIP path has no CPU fallback)")
 
 
-def _dense(t: torch.Tensor):
-    """`t` if its rows are contiguous and do not overlap, else a copy that is such."""
-    return t if t.shape[1] == 1 or t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
-
-
-def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+def _dense(t: torch.Tensor, N: int, n: int):
+    """`t` [N, n] if its rows are contiguous and do not overlap, else a copy that is such."""
+    s0, s1 = t.stride()
+    return t if (s1 == 1 or n == 1) and (s0 >= n or N == 1) else t.contiguous()
 
 
 def _list(t, N: int, device, dtype, name: str, shared: bool = False):
@@ -66,9 +74,14 @@ def _vector(t, N: int, device, dtype, name: str):
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name}: on {t.device}, the logits are on {device}")
-    if tuple(t.shape) != (N,):
+    if t.dim() != 1 or t.shape[0] != N:
         raise ValueError(f"{name}: expected [{N}], got {tuple(t.shape)}")
-    return t.detach().contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _constant(t, name: str):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} gets no gradient: it is a constant here (detach it)")
 
 
 # ---- constraints -----------------------------------------------------------------------------------------------------------------
@@ -85,37 +98,36 @@ def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
     return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32)
 
 
-def _constrain_call(src, dst, logits, lists, backward: bool):
-    a = _lib.Constrain()
-    setattr(a, "in", src.data_ptr())
-    a.out, a.ld_in, a.ld_out = dst.data_ptr(), _ld(src), _ld(dst)
-    if backward:
-        a.logits, a.ld_logits = logits.data_ptr(), _ld(logits)
-    for k, v in lists["fields"].items():
-        setattr(a, k, v.data_ptr() if torch.is_tensor(v) else v)
-    a.type, (a.B, a.V), a.backward = _TYPES[src.dtype], src.shape, int(backward)
-    _lib.check(_lib.load().vln_constrain_logits(C.byref(a), _lib.raw_stream()), "vln_constrain_logits")
+def _constrain_call(src, dst, logits, args, device):
+    """One launch over filled-in `args`; logits: the forward's input (the backward), or None."""
+    setattr(args, "in", src.data_ptr())
+    args.out = dst.data_ptr()
+    args.ld_in, args.ld_out = max(src.stride(0), args.V), max(dst.stride(0), args.V)
+    args.backward = 0
+    if logits is not None:
+        args.logits, args.ld_logits, args.backward = logits.data_ptr(), max(logits.stride(0), args.V), 1
+    _launch(_lib.load().vln_constrain_logits, "vln_constrain_logits", device, _byref(args))
 
 
 class _Constrain(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, lists):
-        z = _dense(logits.detach())
+    def forward(ctx, logits, args, lists):
+        N, V = logits.shape
+        z = _dense(logits, N, V)
         out = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        with _on(z.device):
-            _constrain_call(z, out, None, lists, False)
-        ctx.save_for_backward(logits, *lists["tensors"])         # (a list changed in place before the backward is an error, not a wrong gradient)
-        ctx.lists = lists
+        _constrain_call(z, out, None, args, z.device)
+        ctx.save_for_backward(logits, *lists)         # (a list changed in place before the backward is an error, not a wrong gradient)
+        ctx.args = args
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        z = _dense(ctx.saved_tensors[0].detach())
-        d = _dense(dout.detach())
+        logits = ctx.saved_tensors[0]
+        N, V = logits.shape
+        z, d = _dense(logits, N, V), _dense(dout, N, V)
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        with _on(z.device):
-            _constrain_call(d, dz, z, ctx.lists, True)
-        return dz, None
+        _constrain_call(d, dz, z, ctx.args, z.device)
+        return dz, None, None
 
 
 def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, history_lengths: Optional[torch.Tensor] = None,
@@ -139,88 +151,102 @@ def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = 
 
     out: where to write (same shape and type; `logits` itself: in place, untouched words are not even read).  Without `out` the result
     carries gradients to `logits` (0 for banned words); penalties and biases are constants."""
-    _rows(logits, "constrain_logits")
-    N, V = logits.shape
+    N, V, code = _rows(logits, "constrain_logits")
     dev = logits.device
-    fields, tensors = {}, []
-
-    def put(name, t):
-        fields[name] = t
-        tensors.append(t)
-
-    for name, size, ids, lens in (("history", "H", history, history_lengths), ("prompt", "P", prompt, prompt_lengths)):
-        if ids is None:
-            if lens is not None:
-                raise ValueError(f"constrain_logits: {name}_lengths without {name}")
-            continue
-        t = _list(ids, N, dev, torch.int64, f"constrain_logits: {name}")
-        if t.shape[1] >= 1 << 31:
-            raise ValueError(f"constrain_logits: {name} is longer than 2^31 words")
-        if t.shape[1]:
-            put(name, t)
-            fields[size], fields["ld_" + name] = t.shape[1], t.stride(0)
-            if lens is not None:
-                put(name + "_len", _vector(lens, N, dev, torch.int64, f"constrain_logits: {name}_lengths"))
-    for name, v, low in (("repetition", repetition, 0.0), ("presence", presence, None), ("frequency", frequency, None)):
-        if torch.is_tensor(v):
-            if v.requires_grad and torch.is_grad_enabled():
-                raise ValueError(f"constrain_logits: {name} is a constant, it gets no gradient (detach it)")
-            put(name, _vector(v, N, dev, torch.float32, f"constrain_logits: {name}"))
+    a, lists = _lib.Constrain(), []
+    a.type, a.B, a.V = code, N, V
+    if history is not None:
+        _word_list(a, lists, history, history_lengths, N, dev, "history", "H")
+    elif history_lengths is not None:
+        raise ValueError("constrain_logits: history_lengths without history")
+    if prompt is not None:
+        _word_list(a, lists, prompt, prompt_lengths, N, dev, "prompt", "P")
+    elif prompt_lengths is not None:
+        raise ValueError("constrain_logits: prompt_lengths without prompt")
+    for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if isinstance(v, torch.Tensor):
+            _constant(v, "constrain_logits: " + name)
+            v = _vector(v, N, dev, torch.float32, "constrain_logits: " + name)
+            setattr(a, name, v.data_ptr())
+            lists.append(v)
         else:
             v = float(v)
-            if v != v or abs(v) == float("inf") or low is not None and v <= low:
+            if not abs(v) < float("inf") or name == "repetition" and v <= 0.0:
                 raise ValueError(f"constrain_logits: {name} = {v}")
-            fields[name + "_all"] = v
+            setattr(a, name + "_all", v)
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("constrain_logits: bias_ids and bias_values belong together")
     if bias_ids is not None:
-        if bias_values.requires_grad and torch.is_grad_enabled():
-            raise ValueError("constrain_logits: bias_values are constants, they get no gradient (detach them)")
+        _constant(bias_values, "constrain_logits: bias_values")
         bi = _list(bias_ids, N, dev, torch.int64, "constrain_logits: bias_ids", True)
-        bv = _list(bias_values.detach(), N, dev, torch.float32, "constrain_logits: bias_values", True)
-        if bi.shape != bv.shape or bi.shape[1] > _lib.CONSTRAIN_MAX_BIAS:
+        bv = _list(bias_values, N, dev, torch.float32, "constrain_logits: bias_values", True)
+        n = bi.shape[1]
+        if bv.shape[1] != n or n > _lib.CONSTRAIN_MAX_BIAS:
             raise ValueError(f"constrain_logits: bias_ids {tuple(bias_ids.shape)} and bias_values {tuple(bias_values.shape)} must match, "
                              f"at most {_lib.CONSTRAIN_MAX_BIAS} per row")
-        if bi.shape[1]:
-            put("bias_ids", bi)
-            put("bias_values", bv)
-            fields["n_bias"], fields["ld_bias_ids"], fields["ld_bias_values"] = bi.shape[1], bi.stride(0), bv.stride(0)
-    if allowed is None:
+        if n:
+            a.bias_ids, a.bias_values, a.n_bias, a.ld_bias_ids, a.ld_bias_values = bi.data_ptr(), bv.data_ptr(), n, bi.stride(0), bv.stride(0)
+            lists += (bi, bv)
+    if allowed is not None:
+        words = (V + 31) // 32
+        if allowed.dim() != 2 or allowed.shape[0] < 1 or allowed.shape[1] != words:
+            raise ValueError(f"constrain_logits: allowed must be [G >= 1, {words}] for {V} words, got {tuple(allowed.shape)}")
+        G = allowed.shape[0]
+        al = _dense(_list(allowed, G, dev, torch.int32, "constrain_logits: allowed"), G, words)
+        a.allowed, a.G, a.ld_allowed = al.data_ptr(), G, max(al.stride(0), words)
+        lists.append(al)
         if allowed_rows is not None:
-            raise ValueError("constrain_logits: allowed_rows without allowed")
-    else:
-        if allowed.dim() != 2 or allowed.shape[0] < 1 or allowed.shape[1] != (V + 31) // 32:
-            raise ValueError(f"constrain_logits: allowed must be [G >= 1, {(V + 31) // 32}] for {V} words, got {tuple(allowed.shape)}")
-        al = _dense(_list(allowed, allowed.shape[0], dev, torch.int32, "constrain_logits: allowed"))
-        if allowed_rows is None and al.shape[0] not in (1, N):
-            raise ValueError(f"constrain_logits: {al.shape[0]} mask rows for {N} rows of logits need allowed_rows")
-        put("allowed", al)
-        fields["G"], fields["ld_allowed"] = al.shape[0], _ld(al)
-        if allowed_rows is not None:
-            put("allowed_rows", _vector(allowed_rows, N, dev, torch.int64, "constrain_logits: allowed_rows"))
-    lists = {"fields": fields, "tensors": tensors}
+            rows = _vector(allowed_rows, N, dev, torch.int64, "constrain_logits: allowed_rows")
+            a.allowed_rows = rows.data_ptr()
+            lists.append(rows)
+        elif G != 1 and G != N:
+            raise ValueError(f"constrain_logits: {G} mask rows for {N} rows of logits need allowed_rows")
+    elif allowed_rows is not None:
+        raise ValueError("constrain_logits: allowed_rows without allowed")
+    learns = logits.requires_grad and torch.is_grad_enabled()
     if out is None:
         _gpu(logits, "constrain_logits")
         if N == 0:
             return logits.clone()
-        return _Constrain.apply(logits, lists)
-    if logits.requires_grad and torch.is_grad_enabled() or out.requires_grad:
+        if learns:
+            return _Constrain.apply(logits, a, lists)
+        z = _dense(logits, N, V)
+        out = torch.empty(z.shape, dtype=z.dtype, device=dev)
+        _constrain_call(z, out, None, a, dev)
+        return out
+    if learns or out.requires_grad:
         raise ValueError("constrain_logits: out= carries no gradient; leave it out, or call it under torch.no_grad() on detached logits")
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
         raise ValueError(f"constrain_logits: out must be {tuple(logits.shape)} {logits.dtype} on {dev}")
-    for t, name in ((logits, "logits"), (out, "out")):
-        if N and _dense(t) is not t:
-            raise ValueError(f"constrain_logits: with out=, the rows of {name} must be contiguous and must not overlap")
-    if out.data_ptr() != logits.data_ptr() or _ld(out) != _ld(logits):
-        lo = lambda t: t.data_ptr()
-        hi = lambda t: t.data_ptr() + ((N - 1) * _ld(t) + V) * t.element_size()
-        if N and lo(out) < hi(logits) and lo(logits) < hi(out):
+    if N and (_dense(logits, N, V) is not logits or _dense(out, N, V) is not out):
+        raise ValueError("constrain_logits: with out=, the rows of both tensors must be contiguous and must not overlap")
+    ld_in, ld_out, p_in, p_out = max(logits.stride(0), V), max(out.stride(0), V), logits.data_ptr(), out.data_ptr()
+    if N and not (p_in == p_out and (ld_in == ld_out or N == 1)):
+        size = logits.element_size()
+        if p_out < p_in + ((N - 1) * ld_in + V) * size and p_in < p_out + ((N - 1) * ld_out + V) * size:
             raise ValueError("constrain_logits: out overlaps the logits without being the same tensor")
     _gpu(logits, "constrain_logits")
     if N:
-        with _on(dev):
-            _constrain_call(logits.detach(), out, None, lists, False)
+        _constrain_call(logits, out, None, a, dev)
     return out
+
+
+def _word_list(a, lists, ids, lens, N, dev, name, size):
+    """history / prompt: the struct's <name>, ld_<name>, <name>_len and the length H / P."""
+    t = _list(ids, N, dev, torch.int64, "constrain_logits: " + name)
+    n = t.shape[1]
+    if n >= 1 << 31:
+        raise ValueError(f"constrain_logits: {name} is longer than 2^31 words")
+    if lens is not None:
+        lens = _vector(lens, N, dev, torch.int64, f"constrain_logits: {name}_lengths")
+    if n:
+        setattr(a, name, t.data_ptr())
+        setattr(a, "ld_" + name, t.stride(0))
+        setattr(a, size, n)
+        lists.append(t)
+        if lens is not None:
+            setattr(a, name + "_len", lens.data_ptr())
+            lists.append(lens)
 
 
 # ---- a teacher's top logits ------------------------------------------------------------------------------------------------------
@@ -231,83 +257,85 @@ def _temperature(T, who):
     return T
 
 
+@functools.lru_cache(maxsize=4096)
+def _top_ws(device_index, N, V, code, k):          # (depends on the device's number of compute units)
+    return _lib.load().vln_top_logits_ws_bytes(N, V, code, k)
+
+
+@functools.lru_cache(maxsize=4096)
+def _distill_ws(device_index, N, V, code):
+    return _lib.load().vln_distill_ws_bytes(N, V, code)
+
+
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     """(values [N, k], ids [N, k] int64, rest [N] float32): the k largest logits of every row, largest first, equal ones in the order of
     their ids (NaN counts as largest), and `rest = logsumexp(all other logits / temperature)` (-inf: none) -- the targets that
     `distill_loss` takes; `ids` with k = 1 is the greedy word.  1 <= k <= min(V, 256).  No gradient: a teacher is a constant."""
-    _rows(logits, "top_logits")
+    N, V, code = _rows(logits, "top_logits")
     T = _temperature(temperature, "top_logits")
-    N, V = logits.shape
     k = int(k)
     if not 1 <= k <= min(V, _lib.TOP_LOGITS_MAX):
         raise ValueError(f"top_logits: k = {k} outside 1 .. {min(V, _lib.TOP_LOGITS_MAX)}")
     _gpu(logits, "top_logits")
-    z = _dense(logits.detach())
+    z = _dense(logits, N, V)
     dev = z.device
     values = torch.empty(N, k, dtype=z.dtype, device=dev)
     ids = torch.empty(N, k, dtype=torch.int64, device=dev)
     rest = torch.empty(N, dtype=torch.float32, device=dev)
     if N:
-        lib = _lib.load()
-        with _on(dev):
-            nb = lib.vln_top_logits_ws_bytes(N, V, _TYPES[z.dtype], k)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-            _lib.check(lib.vln_top_logits(z.data_ptr(), _ld(z), _TYPES[z.dtype], N, V, k, T, values.data_ptr(), ids.data_ptr(), rest.data_ptr(),
-                                          _p(ws), nb, _lib.raw_stream()), "vln_top_logits")
+        nb = _top_ws(dev.index, N, V, code, k)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        _launch(_lib.load().vln_top_logits, "vln_top_logits", dev, z.data_ptr(), max(z.stride(0), V), code, N, V, k, T, values.data_ptr(),
+                ids.data_ptr(), rest.data_ptr(), ws.data_ptr() if nb else None, nb)
     return values, ids, rest
 
 
 # ---- distillation ----------------------------------------------------------------------------------------------------------------
-def _grad_like(z: torch.Tensor):
+def _grad_like(z: torch.Tensor, N: int, V: int):
     """An uninitialised gradient for the rows `z`: where a row's distance from a 16-byte boundary changes from row to row (an odd
     vocabulary), the gradient's rows get the same distances, so that reads and writes can both take 16 bytes."""
-    N, V = z.shape
-    per = 16 // z.element_size()
-    pad = (_ld(z) - V) % per
+    pad = (max(z.stride(0), V) - V) % (16 // z.element_size())
     return torch.empty(N, V + pad, dtype=z.dtype, device=z.device)[:, :V] if pad else torch.empty(N, V, dtype=z.dtype, device=z.device)
+
+
+def _distill_forward(z, N, V, code, ids, teacher, rest, target, T, alpha, ignore_index, red):
+    """(loss, the filled-in struct, what it points to besides the inputs): the struct serves the backward as well."""
+    dev = z.device
+    # one buffer: the rows' statistics (16-byte aligned), 1 / count, and the rows' losses unless they are the result
+    own_rows = N if red else 0
+    buf = torch.empty(N * _lib.DISTILL_STATS + 4 + own_rows, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev) if red else torch.empty(N, dtype=torch.float32, device=dev)
+    stats, out = buf.data_ptr(), loss.data_ptr()
+    inv = stats + 4 * N * _lib.DISTILL_STATS
+    K = ids.shape[1]
+    a = _lib.Distill(z.data_ptr(), max(z.stride(0), V), ids.data_ptr(), max(ids.stride(0), K), teacher.data_ptr(), max(teacher.stride(0), K),
+                     None if rest is None else rest.data_ptr(), None if target is None else target.data_ptr(), ignore_index,
+                     inv + 16 if red else out, stats, T, alpha, code, _TYPES[teacher.dtype], N, V, K, 0)
+    nb = _distill_ws(dev.index, N, V, code)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    _launch(_lib.load().vln_distill_fwd, "vln_distill_fwd", dev, _byref(a), red, out if red else None, inv if red else None,
+            ws.data_ptr() if nb else None, nb)
+    return loss, a, (z, buf, inv if red else None)
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, ids, teacher, rest, target, T, alpha, ignore_index, reduction):
-        z = _dense(logits.detach())
-        N, V = z.shape
-        dev = z.device
-        lib = _lib.load()
-        red = _lib.REDUCE[reduction]
-        f32 = dict(dtype=torch.float32, device=dev)
-        rows, stats = torch.empty(N, **f32), torch.empty(N, _lib.DISTILL_STATS, **f32)
-        out = torch.empty(2, **f32) if red else None                # [loss, what the backward multiplies with]
-        with _on(dev):
-            a = _Distill.args(z, ids, teacher, rest, target, T, alpha, ignore_index, rows, stats)
-            nb = lib.vln_distill_ws_bytes(N, V, a.type)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-            _lib.check(lib.vln_distill_fwd(C.byref(a), red, _p(out), _p(ws), nb, _lib.raw_stream()), "vln_distill_fwd")
-        ctx.save_for_backward(logits, ids, teacher, rest, target, rows, stats, out)
-        ctx.cfg = (T, alpha, ignore_index, red)
-        return out[0] if red else rows
-
-    @staticmethod
-    def args(z, ids, teacher, rest, target, T, alpha, ignore_index, rows, stats):
-        return _lib.Distill(z.data_ptr(), _ld(z), ids.data_ptr(), _ld(ids), teacher.data_ptr(), _ld(teacher), _p(rest), _p(target),
-                            ignore_index, rows.data_ptr(), stats.data_ptr(), T, alpha, _TYPES[z.dtype], _TYPES[teacher.dtype], z.shape[0],
-                            z.shape[1], ids.shape[1], 0)
+    def forward(ctx, logits, meta):
+        N, V, _, ids, teacher, rest, target = meta[:7]
+        loss, ctx.args, ctx.keep = _distill_forward(_dense(logits, N, V), *meta)
+        ctx.save_for_backward(logits, ids, teacher, rest, target)     # (one of them changed in place before the backward is an error)
+        return loss
 
     @staticmethod
     def backward(ctx, dloss):
-        logits, ids, teacher, rest, target, rows, stats, out = ctx.saved_tensors
-        T, alpha, ignore_index, red = ctx.cfg
-        z = _dense(logits.detach())
-        dz = _grad_like(z)
-        if red or dloss.stride(0) == 0:
-            stride = 0
-        else:
+        ctx.saved_tensors
+        a, (z, _buf, inv) = ctx.args, ctx.keep
+        dz = _grad_like(z, a.N, a.V)
+        stride = 0
+        if inv is None and dloss.stride(0) != 0:
             stride, dloss = 1, dloss.contiguous()
-        with _on(z.device):
-            a = _Distill.args(z, ids, teacher, rest, target, T, alpha, ignore_index, rows, stats)
-            _lib.check(_lib.load().vln_distill_bwd(C.byref(a), dloss.data_ptr(), stride, out.data_ptr() + 4 if red else None, dz.data_ptr(),
-                                                   dz.stride(0), _lib.raw_stream()), "vln_distill_bwd")
-        return dz, None, None, None, None, None, None, None, None
+        _launch(_lib.load().vln_distill_bwd, "vln_distill_bwd", z.device, _byref(a), dloss.data_ptr(), stride, inv, dz.data_ptr(), dz.stride(0))
+        return dz, None
 
 
 def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_values: torch.Tensor, *, teacher_rest: Optional[torch.Tensor] = None,
@@ -329,30 +357,35 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_values
 
     One pass over the logits forward, one backward (logits in, gradient out); nothing of size [N, V] is kept in between.  Gradients go
     to `logits` only."""
-    _rows(logits, "distill_loss")
-    N, V = logits.shape
+    N, V, code = _rows(logits, "distill_loss")
     dev = logits.device
     T = _temperature(temperature, "distill_loss")
     alpha = float(alpha)
     if not 0.0 <= alpha <= 1.0:
         raise ValueError(f"distill_loss: alpha {alpha} outside [0, 1]")
-    if reduction not in _lib.REDUCE:
+    red = _lib.REDUCE.get(reduction)
+    if red is None:
         raise ValueError("distill_loss: reduction must be 'none', 'sum' or 'mean'")
-    if target is None and alpha < 1.0:
-        raise ValueError("distill_loss: alpha < 1 needs targets")
-    for t, name in ((teacher_values, "teacher_values"), (teacher_rest, "teacher_rest")):
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"distill_loss: {name} is a constant, it gets no gradient (detach it)")
-    ids = _list(teacher_ids, N, dev, torch.int64, "distill_loss: teacher_ids")
     if teacher_values.dtype not in _TYPES:
         raise TypeError(f"distill_loss: teacher_values must be float32 or bfloat16, got {teacher_values.dtype}")
-    tv = _list(teacher_values.detach(), N, dev, teacher_values.dtype, "distill_loss: teacher_values")
-    if ids.shape != tv.shape or not 1 <= ids.shape[1] <= _lib.DISTILL_MAX:
+    _constant(teacher_values, "distill_loss: teacher_values")
+    ids = _list(teacher_ids, N, dev, torch.int64, "distill_loss: teacher_ids")
+    tv = _list(teacher_values, N, dev, teacher_values.dtype, "distill_loss: teacher_values")
+    K = ids.shape[1]
+    if tv.shape[1] != K or not 1 <= K <= _lib.DISTILL_MAX:
         raise ValueError(f"distill_loss: teacher_ids {tuple(ids.shape)} and teacher_values {tuple(tv.shape)} must match, 1 .. {_lib.DISTILL_MAX} per row")
-    ids, tv = _dense(ids), _dense(tv)
-    rest = None if teacher_rest is None else _vector(teacher_rest, N, dev, torch.float32, "distill_loss: teacher_rest")
-    tgt = None if target is None else _vector(target, N, dev, torch.int64, "distill_loss: target")
+    ids, tv = _dense(ids, N, K), _dense(tv, N, K)
+    if teacher_rest is not None:
+        _constant(teacher_rest, "distill_loss: teacher_rest")
+        teacher_rest = _vector(teacher_rest, N, dev, torch.float32, "distill_loss: teacher_rest")
+    if target is not None:
+        target = _vector(target, N, dev, torch.int64, "distill_loss: target")
+    elif alpha < 1.0:
+        raise ValueError("distill_loss: alpha < 1 needs targets")
     _gpu(logits, "distill_loss")
     if N == 0:
         return logits.float().sum(1) if reduction == "none" else logits.float().sum() * (1.0 if reduction == "sum" else float("nan"))
-    return _Distill.apply(logits, ids, tv, rest, tgt, T, alpha, int(ignore_index), reduction)
+    meta = (N, V, code, ids, tv, teacher_rest, target, T, alpha, int(ignore_index), red)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Distill.apply(logits, meta)
+    return _distill_forward(_dense(logits, N, V), *meta)[0]

@@ -390,8 +390,8 @@ int vln_top_logits(const void* logits, int64_t ld, int type, int N, int V, int k
  * A word listed twice: two outcomes that share a word.  A row whose target is ignore_index -- without targets, a row whose teacher has
  * no mass -- has loss 0 and gradient 0 and is not counted by the mean (no row counted: NaN); any other target outside [0, V) makes its
  * row NaN.  With targets, a row whose teacher has no mass keeps its hard term.  alpha < 1 needs targets.
- * rows [N] receives the row losses, stats [N, VLN_DISTILL_STATS] what the backward needs, out[0] the loss and out[1] the factor that the
- * backward takes as inv_count (reduction != VLN_REDUCE_NONE).  ws: vln_distill_ws_bytes (0: may be NULL). */
+ * rows [N] receives the row losses, stats [N, VLN_DISTILL_STATS] (16-byte aligned) what the backward needs; with a reduction, loss [1]
+ * and the factor inv_count [1] that the backward takes.  ws: vln_distill_ws_bytes (0: may be NULL), 16-byte aligned. */
 #define VLN_DISTILL_MAX 256
 #define VLN_DISTILL_STATS 12
 #define VLN_REDUCE_NONE 0
@@ -408,8 +408,8 @@ typedef struct vln_distill {
   int32_t type, teacher_type, N, V, K, pad_;
 } vln_distill;
 int64_t vln_distill_ws_bytes(int N, int V, int type);
-int vln_distill_fwd(const vln_distill* args, int reduction, float* out, void* ws, int64_t ws_bytes, vln_stream_t s);
-/* dloss_stride 1: one upstream gradient per row, 0: one for all; inv_count: the forward's out + 1 (NULL: 1) */
+int vln_distill_fwd(const vln_distill* args, int reduction, float* loss, float* inv_count, void* ws, int64_t ws_bytes, vln_stream_t s);
+/* dloss_stride 1: one upstream gradient per row, 0: one for all; inv_count: the forward's (NULL: 1); rows is not used */
 int vln_distill_bwd(const vln_distill* args, const float* dloss, int64_t dloss_stride, const float* inv_count, void* dlogits,
                     int64_t ld_dlogits, vln_stream_t s);
 

@@ -138,7 +138,7 @@ def test_c_abi_refusals(vln):
                 setattr(a, k, v)
         if bwd:
             return lib.vln_distill_bwd(C.byref(a), kw.get("g", p), kw.get("gs", 0), None, kw.get("dz", p), kw.get("ldz", 40), None)
-        return lib.vln_distill_fwd(C.byref(a), kw.get("red", 0), kw.get("out", None), kw.get("ws", None), 0, None)
+        return lib.vln_distill_fwd(C.byref(a), kw.get("red", 0), kw.get("out", None), kw.get("out", None), kw.get("ws", None), 0, None)
 
     for kw in (dict(N=0), dict(V=0), dict(logits=None), dict(ld=3), dict(K=0), dict(K=257, ld_ids=300, ld_teacher=300), dict(ids=None), dict(ld_ids=2), dict(type=2),
                dict(teacher_type=5), dict(temperature=0.0), dict(temperature=float("inf")), dict(alpha=0.5), dict(alpha=2.0, target=p), dict(rows=None),
@@ -147,4 +147,4 @@ def test_c_abi_refusals(vln):
         assert b"vln_distill_fwd" in lib.vln_last_error_string()
     for kw in (dict(g=None), dict(gs=2), dict(dz=None), dict(ldz=39)):
         assert distill(True, **kw) == 1, kw
-    assert lib.vln_distill_fwd(None, 0, None, None, 0, None) == 1
+    assert lib.vln_distill_fwd(None, 0, None, None, None, 0, None) == 1
