@@ -9,8 +9,10 @@
 //      sum) of exp(z / T) -- the others' mass is a sum of positive terms, never a difference;
 //   3. a candidate's place is the number of larger ones; places from k on belong to the others.
 // Elements are ordered by (order-preserving bits of the value, lower index first): all distinct, so ties fall to the lowest index and the
-// order in which candidates were collected does not show.  Where more reach the bound than the list holds (constant or masked rows), the
-// exact border is found by bisection over value and index.  Segments leave their k best, and one workgroup per row selects among them.
+// order in which candidates were collected does not show.  Where more reach the bound than a list holds, or the bound is -inf (rows with
+// fewer words allowed than asked for), the elements above the bound and, in index order, as many equal to it as are missing are taken
+// (their places from a scan of the counts); only if those above are too many as well is the border itself searched by bisection.
+// Segments leave their candidates, and one workgroup per row selects among them.
 #include "word_rows.h"
 #include "../../include/vln_hip.h"
 
@@ -126,8 +128,8 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   __shared__ alignas(16) u64 cand[W * CAP];                   // (first: {value bits, column}, a list per wave)
   __shared__ int place[T];
   __shared__ unsigned gmax[T * G];
-  __shared__ int counts[W], redo, part[2][W];
-  __shared__ float bound;
+  __shared__ int counts[W], redo, part[2][W], gt_n[W], eq_n[NVR * W];
+  __shared__ unsigned bound;
   __shared__ float2 sums[W];
   const long n = blockIdx.x;
   const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -169,40 +171,34 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
       most = max(most, gm[i]);
       least = min(least, gm[i] - 1u);          // (0 - 1: an empty group)
     }
-    float t = __builtin_nanf("");              // fewer groups than k: every element is a candidate
-    if (groups >= a.k) {
-      const unsigned th = bisect_near(wave_umin(least) + 1u, wave_umax(most), a.k, a.k + a.k / 8 + 2, 12, [&](unsigned b) {
+    unsigned th = 0u;                          // fewer groups than k: every element is a candidate
+    if (groups >= a.k)
+      th = bisect_near(wave_umin(least) + 1u, wave_umax(most), a.k, a.k + a.k / 8 + 2, 12, [&](unsigned b) {
         int c = 0;
 #pragma unroll
         for (int i = 0; i < W * G; ++i) c += gm[i] >= b ? 1 : 0;
         return wave_isum(c);
       });
-      t = order_value(th == 0x80000000u ? th - 2 : th - 1);      // just below th (below +0 comes -0, which compares equal to it)
-    }
-    if (lane == 0) bound = t;
+    if (lane == 0) bound = th;
   }
   __syncthreads();
-  const float tval = bound;
+  unsigned border = bound;                     // candidates reach it: !(x <= tval), tval just below (below +0 comes -0, which compares equal)
+  const float tval = border == 0u ? __builtin_nanf("") : order_value(border == 0x80000000u ? border - 2 : border - 1);
+  constexpr unsigned kNegInf = 0x007fffffu;    // order bits of -inf
+  int len = 0;                                 // this wave's list
+  uint2* list = reinterpret_cast<uint2*>(cand) + w * CAP;
   // The others' sum.  Every element that is no candidate is at most ref = min(the thread's largest, the bound), so the exponentials are
   // taken relative to ref, one fused multiply-add each (the rounding of ref * c is taken out again at the end).  Where that is no good
   // reference -- not finite, or everything below it underflows -- the sweep is repeated with a running maximum (`slow`).
   OnlineSum others;
   float ref = fminf(tmax, tval);
-  bool slow = __ballot(!(fabsf(ref) < 1e30f) && ref != -INFINITY) != 0;
+  bool slow = __ballot(!(fabsf(ref) < 1e30f) && ref != -INFINITY) != 0, redone = false;
   if (!(fabsf(ref) < 1e30f)) ref = 0.f;
   const float nm = -ref * a.c, cut_off = fmaf(ref, a.c, nm);
-  bool redone = false;
-  bool exact = false;                          // only elements of order bits > th, or == th and complemented index >= tl, are candidates
-  unsigned th = 0u, tl = 0u;
   constexpr int UV = 8 / VEC;                  // vectors of 8 elements
-  while (true) {
-    int len = 0;                               // this wave's list
-    uint2* list = reinterpret_cast<uint2*>(cand) + w * CAP;
-    auto wanted = [&](float x, int col) {      // of an element above the bound
-      if (!exact) return true;
-      const unsigned o = order_bits(x);
-      return o > th || (o == th && ~(unsigned)col >= tl);
-    };
+  bool full = border == kNegInf;
+  while (!full) {
+    len = 0;
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < NVR; u += UV) {
@@ -218,12 +214,11 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
 #pragma unroll
       for (int j = 1; j < 8; ++j) mx = nan_max(mx, x[j]);
       if (__ballot(!(mx <= tval))) {
-int mine = 0, total;
+        int mine = 0, total;
         bool in[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int iv = i + j / VEC * T;
-          in[j] = !(x[j] <= tval) && iv < v1 && wanted(x[j], g.head + iv * VEC + j % VEC);
+          in[j] = !(x[j] <= tval) && i + j / VEC * T < v1;
           mine += in[j] ? 1 : 0;
         }
         int at = len - mine + wave_scan(mine, total);
@@ -246,7 +241,7 @@ int mine = 0, total;
     }
     if (!slow) {
       if (sum != 0.f) { others.m = ref; others.s = sum * exp2_hw(-cut_off); }
-      if (sum < 1e-30f) {                       // masked words only, or an underflow?
+      if (sum < 1e-30f && tmax != -INFINITY) {  // candidates and masked words only, or an underflow?
         for (int u = v0 + tid; u < v1; u += T) {
           float x[VEC];
           unpack16<E>(ld_vec<E>(p + g.head + (int64_t)u * VEC), x);
@@ -255,7 +250,7 @@ int mine = 0, total;
       }
     }
     if (s == 0) {
-      const bool in = scol >= 0 && !(sx <= tval) && wanted(sx, scol);
+      const bool in = scol >= 0 && !(sx <= tval);
       int total;
       const int at = len - 1 + wave_scan(in ? 1 : 0, total);
       len += total;
@@ -264,42 +259,112 @@ int mine = 0, total;
     }
     if (lane == 0) counts[w] = len;
     __syncthreads();
-    bool full = false;
 #pragma unroll
     for (int i = 0; i < W; ++i) full = full || counts[i] > CAP;
     const bool again = redo != 0 && !redone;   // (the same in every wave; `slow` may differ)
-    if (!full && !again) break;
-    if (again) slow = redone = true;
+    if (full || !again) break;
+    slow = redone = true;
     others = OnlineSum();
     __syncthreads();
-    if (!full) continue;
-    // More reach the bound than the list holds: the exact border, counting the segment's elements per step (read again, from the caches).
-    int turn = 0;
-    auto block_count = [&](auto&& has) {       // has(order bits, complemented index)
-      int c = 0;
-      for (int i = v0 + tid; i < v1; i += T) {
-        float x[VEC];
-        unpack16<E>(ld_vec<E>(p + g.head + (int64_t)i * VEC), x);
-        for (int j = 0; j < VEC; ++j) c += has(order_bits(x[j]), ~(unsigned)(g.head + i * VEC + j)) ? 1 : 0;
-      }
-      if (scol >= 0) c += has(order_bits(sx), ~(unsigned)scol) ? 1 : 0;
+  }
+  if (full) {
+    // The rare forms, in loops over the vectors in memory (the caches hold them).  Nothing but -inf: the first k columns.  Otherwise the
+    // elements above the border and, in index order, the first `need` equal to it.
+    others = OnlineSum();
+    __syncthreads();
+    if (tid == 0) redo = 0;
+    __syncthreads();
+    auto each = [&](int u, auto&& f) {       // f(element, column) of this thread's vector u
+      const int i = v0 + u * T + tid;
+      if (i >= v1) return;
+      float x[VEC];
+      unpack16<E>(ld_vec<E>(p + g.head + (int64_t)i * VEC), x);
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-      if (lane == 0) part[turn][w] = c;
-      __syncthreads();
-      c = 0;
-      for (int i = 0; i < W; ++i) c += part[turn][i];
-      turn ^= 1;
-      return c;
+      for (int j = 0; j < VEC; ++j) f(x[j], g.head + i * VEC + j);
     };
-    bool enough;
-    th = bisect(1u, 0xffffffffu, a.k, enough, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
-    if (!enough) {
-      const int need = a.k - block_count([&](unsigned h, unsigned) { return h > th; });
-      bool e;
-      tl = bisect(0u, 0xffffffffu, need, e, [&](unsigned t) { return block_count([&](unsigned h, unsigned l) { return h == th && l >= t; }); });
+    bool other = sx != -INFINITY;
+#pragma unroll 4
+    for (int u = 0; u < NVR; ++u) each(u, [&](float x, int) { other = other || x != -INFINITY; });
+    if (__ballot(other) && lane == 0) redo = 1;
+    __syncthreads();
+    if (!redo) {
+      const int c0 = s == 0 ? 0 : g.head + v0 * VEC, n_col = (v1 - v0) * VEC + (s == 0 ? g.head + g.tail : 0);
+      len = w == 0 ? min(a.k, n_col) : 0;
+      for (int c = lane; c < len; c += 64) {
+        const int body = g.head + (v1 - v0) * VEC;
+        list[c] = make_uint2(0xff800000u, s == 0 && c >= body ? g.tail0() + c - body : c0 + c);
+      }
+    } else {
+      int turn = 0;
+      auto block_count = [&](unsigned t) {     // elements of the segment with order bits >= t
+        int c = scol >= 0 && order_bits(sx) >= t ? 1 : 0;
+#pragma unroll 2
+        for (int u = 0; u < NVR; ++u) each(u, [&](float x, int) { c += order_bits(x) >= t ? 1 : 0; });
+        c = wave_isum(c);
+        if (lane == 0) part[turn][w] = c;
+        __syncthreads();
+        c = 0;
+        for (int i = 0; i < W; ++i) c += part[turn][i];
+        turn ^= 1;
+        return c;
+      };
+      int above;
+      for (int go = 0; go < 2; ++go) {
+        // above the border, per wave, and equal to it, per vector and wave: index order is head, vectors by (u, wave, lane), tail
+        int gt = scol >= 0 && order_bits(sx) > border ? 1 : 0;
+#pragma unroll 2
+        for (int u = 0; u < NVR; ++u) {
+          int eq = 0;
+          each(u, [&](float x, int) { const unsigned o = order_bits(x); gt += o > border ? 1 : 0; eq += o == border ? 1 : 0; });
+          eq = wave_isum(eq);
+          if (lane == 0) eq_n[u * W + w] = eq;
+        }
+        gt = wave_isum(gt);
+        if (lane == 0) gt_n[w] = gt;
+        __syncthreads();
+        above = 0;
+        bool many = false;
+        for (int i = 0; i < W; ++i) { above += gt_n[i]; many = many || gt_n[i] > CAP; }
+        if (!many || above < a.k) break;       // (fewer than k above: k in all, which a list holds)
+        bool exact;                            // too many above it as well: the k-th largest value itself (fewer than k above)
+        border = bisect(border + 1u, 0xffffffffu, a.k, exact, block_count);
+        __syncthreads();
+      }
+      const int need = max(0, a.k - above);
+      int eq_head = 0;
+      if (s == 0) for (int c = 0; c < g.head; ++c) eq_head += order_bits(Elt<E>::ld(p + c)) == border ? 1 : 0;
+      int eq_before = eq_head;
+      len = 0;
+      for (int u = 0; u < NVR; ++u) {
+        int eq = 0, all;
+        each(u, [&](float x, int) { eq += order_bits(x) == border ? 1 : 0; });
+        int before = eq_before - eq + wave_scan(eq, all);
+        for (int q = 0; q < W; ++q) { const int c = eq_n[u * W + q]; eq_before += c; if (q < w) before += c; }
+        int mine = 0, rank = before;
+        auto in = [&](float x) { const unsigned o = order_bits(x); return o > border || (o == border && rank++ < need); };
+        each(u, [&](float x, int) { mine += in(x) ? 1 : 0; });
+        int at = len - mine + wave_scan(mine, all);
+        len += all;
+        rank = before;
+        each(u, [&](float x, int col) {
+          if (in(x)) list[at++] = make_uint2(__float_as_uint(x), col);
+          else others.add1(x, a.c);
+        });
+      }
+      if (s == 0) {
+        const unsigned o = order_bits(sx);
+        const bool tail = scol >= g.head;
+        int all;
+        const int before = wave_scan(scol >= 0 && o == border ? 1 : 0, all) - 1 - (tail ? eq_head : 0) + (tail ? eq_before : 0);
+        const bool in = scol >= 0 && (o > border || (o == border && before < need));
+        const int at = len - 1 + wave_scan(in ? 1 : 0, all);
+        len += all;
+        if (in) list[at] = make_uint2(__float_as_uint(sx), scol);
+        else if (scol >= 0) others.add1(sx, a.c);
+      }
     }
-    exact = slow = redone = true;              // (others may now lie above the bound)
+    if (lane == 0) counts[w] = len;
+    __syncthreads();
   }
   // the waves' lists as one list of keys, in a fixed order
   int nc = 0, before = 0;

@@ -298,6 +298,26 @@ def test_top_logits_orders_and_ties(vocab, V, k):
     check_top(vocab, z.to(torch.bfloat16), k, 2.0)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("N,V,k", [(3, 992, 16), (4, 5003, 256), (2, 70001, 64), (600, 2500, 40), (2, 70001, 1)])
+def test_top_logits_of_masked_rows(vocab, N, V, k, dt):
+    """Rows in which a grammar left fewer words than are asked for, or a few in one place, or none: equal values (-inf, 0) fill the rest in
+    index order, across vectors, waves and segments."""
+    g = torch.Generator().manual_seed(V + k)
+    z = torch.randn(N, V, generator=g).to(DT[dt])
+    for b in range(N):
+        left = [0, 1, k // 2, 2 * k, V // 50][b % 5]
+        keep = torch.randperm(V, generator=g)[:left] if b % 2 else torch.arange(V // 3, min(V, V // 3 + left))
+        m = torch.full((V,), NINF, dtype=z.dtype)
+        m[keep] = z[b, keep]
+        z[b] = m
+    z[-1] = torch.where(torch.isinf(z[-1]), torch.zeros_like(z[-1]), z[-1].abs())      # ties at a finite value
+    check_top(vocab, z, k, 1.0)
+    check_top(vocab, z, k, 2.0, "odd")
+    quantised = (torch.randn(N, V, generator=g) * 2).round().to(DT[dt])                # a dozen different values
+    check_top(vocab, quantised, k, 1.0, "odd")
+
+
 def test_top_logits_nan_and_infinities(vocab):
     V = 3000
     g = torch.Generator().manual_seed(4)
