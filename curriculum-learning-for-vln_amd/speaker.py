@@ -422,11 +422,28 @@ class Speaker:
     def _zero_state(self, B, dev):
         return (torch.zeros(1, B, self.rnn_dim, device=dev), torch.zeros(1, B, self.rnn_dim, device=dev))
 
-    def teacher_forcing(self, can_feats, img_feats, lengths, insts, train: bool = True, for_listener: bool = False, ctx_mask=None):
+    def teacher_targets(self, can_feats, img_feats, lengths, insts, k: int = 16, temperature: float = 2.0, alpha: float = 0.5, ctx_mask=None):
+        """This speaker as a TEACHER: its k largest word logits at every position of `insts` and the log-mass of the other words, as the
+        `vocab.DistillTargets` that a student's `teacher_forcing(distill=...)` takes (rows b * Lw + t).  Evaluation mode, no gradient."""
+        from . import vocab
+        self._mode(False)
+        with torch.no_grad():
+            ctx = self.encoder(can_feats, img_feats, lengths)
+            if ctx_mask is None:
+                ctx_mask = length2mask(lengths, can_feats.device, ctx.shape[1])
+            logits, _, _ = self.decoder(insts, ctx, ctx_mask, *self._zero_state(can_feats.shape[0], can_feats.device))
+            values, ids, rest = vocab.top_logits(logits.reshape(-1, logits.shape[2]), k, temperature)
+        return vocab.DistillTargets(ids, values, rest, float(temperature), float(alpha))
+
+    def teacher_forcing(self, can_feats, img_feats, lengths, insts, train: bool = True, for_listener: bool = False, ctx_mask=None, distill=None):
         """speaker.py:235-290.  insts [B, Lw] int64 (<BOS> w1 .. <EOS> <PAD>..).  train -> mean CE over the non-pad
         targets; for_listener -> the un-reduced [B, Lw-1] losses (beam-search scoring); eval -> (loss, word_accu,
-        sent_accu).  ctx_mask: `length2mask(lengths)` already on the device (a captured iteration cannot copy it there)."""
+        sent_accu).  ctx_mask: `length2mask(lengths)` already on the device (a captured iteration cannot copy it there).
+        distill (a vocab.DistillTargets over the same words; train only): the mean of alpha * T^2 * KL(teacher || this speaker) +
+        (1 - alpha) * CE over the non-pad targets instead of the mean CE (vocab.distill_loss)."""
         from . import losses
+        if distill is not None and (not train or for_listener):
+            raise ValueError("Speaker.teacher_forcing: distill belongs to training (train=True, for_listener=False)")
         self._mode(train)
         dev = can_feats.device
         B = can_feats.shape[0]
@@ -440,6 +457,10 @@ class Speaker:
         # last one against <PAD> -- ignored by the loss, zero gradient, exactly what the slice's backward would have filled in
         flat = logits.reshape(B * Lw, V)
         tgt = torch.cat((insts[:, 1:], insts.new_full((B, 1), self.pad)), 1).reshape(-1)
+        if distill is not None:
+            from . import vocab
+            return vocab.distill_loss(flat, distill.ids, distill.values, teacher_rest=distill.rest, temperature=distill.temperature, target=tgt,
+                                      alpha=distill.alpha, ignore_index=self.pad)
         if train and not for_listener:             # mean over the non-pad targets inside the launch (speaker.py:272-273)
             return losses.masked_cross_entropy(flat, tgt, None, "mean", ignore_index=self.pad)
         per_word = losses.masked_cross_entropy(flat, tgt, None, "none", ignore_index=self.pad).view(B, Lw)[:, :-1]
@@ -455,10 +476,12 @@ class Speaker:
         sent_accu = (correct.sum(dim=1) == n_gt).sum().item() / B
         return loss.item(), word_accu, sent_accu
 
-    def infer_batch(self, can_feats, img_feats, lengths, sampling: bool = False, train: bool = False, featdropmask=None):
+    def infer_batch(self, can_feats, img_feats, lengths, sampling: bool = False, train: bool = False, featdropmask=None, constraints=None):
         """speaker.py:292-376.  Greedy (or sampled) decoding from <BOS> until every row has produced <EOS> or
         `max_decode` words; words after a row's <EOS> are <PAD>.  `featdropmask` [F-angle]: the environment-dropout
         mask shared with the follower (applied in place to the image part of both feature tensors, speaker.py:313-315).
+        `constraints` (vocab.WordConstraints): penalties for repeated words, word biases and a grammar's masks on every word's logits, the
+        words so far being the history; <UNK> stays banned.  A grammar that allows no word at all draws word 0.
         Returns words [B, n] (numpy int64); with sampling and train also (log_probs, hiddens, entropies) as tensors
         that carry gradients."""
         import numpy as np
@@ -478,19 +501,30 @@ class Speaker:
         unk_mask = torch.zeros(B, self.decoder.projection.out_features, dtype=torch.bool, device=dev)
         unk_mask[:, self.unk] = True                                                  # no <UNK> in inference (speaker.py:336)
         words, log_probs, hiddens, entropies = [], [], [], []
+        if constraints is not None:
+            from . import vocab
+            constraints = constraints.banning(self.unk, B, dev)
+            said = torch.empty(B, self.max_decode, dtype=torch.int64, device=dev)      # the words fed back, the history of the next one
         grad = torch.enable_grad() if (train and sampling) else torch.no_grad()
         with grad:
-            for _ in range(self.max_decode):
+            for t in range(self.max_decode):
                 logits, h_t, c_t = self.decoder(word, ctx, ctx_mask, h_t, c_t)        # [B, 1, vocab]
                 logits = logits.view(B, -1)
+                if constraints is not None:
+                    # (a copy where a backward will need it: the buffer is written below)
+                    logits = constraints.apply(logits, said[:, :t].clone() if logits.requires_grad else said[:, :t])
                 if sampling:
                     self._draws += 1
                     w, lp, ent = losses.sample_action(logits, unk_mask, seed=self.seed, offset=self._draws)
                     log_probs.append(lp if train else lp.detach())
                     hiddens.append(h_t.squeeze(0) if train else h_t.squeeze(0).detach())
                     entropies.append(ent if train else ent.detach())
+                elif constraints is not None:
+                    w = vocab.top_logits(logits, 1)[1].view(B)
                 else:
                     w = logits.masked_fill(unk_mask, float("-inf")).argmax(dim=1)
+                if constraints is not None:
+                    said[:, t] = w
                 cpu_word = w.cpu().numpy().copy()          # a COPY: the word fed back below keeps the model's choice
                 cpu_word[ended] = self.pad
                 words.append(cpu_word)

@@ -24,7 +24,7 @@ import time
 
 import torch
 
-from . import _lib, dp, functional, losses, ops, optim
+from . import _lib, dp, functional, losses, ops, optim, vocab
 from .decoders import AttnDecoderLSTM, MonitorDecoder
 from .encoder import EncoderLSTM
 from .envdrop_decoder import Critic, EnvDropDecoder
@@ -630,13 +630,18 @@ class SpeakerIteration(_GraphedIteration):
     batch: `can` [B, Lp, F] (the taken views), `img` [B, Lp, 36, F], `lengths` [B] (CPU), `insts` [B, Lw].
     graph=True (round 6): dropout offsets and the three recurrences' launch sequences come from a runtime.DeviceClock, the batch
     lives at fixed addresses (`load`: also the path mask, which the eager form builds on the host every iteration), and
-    `capture()` / `replay()` run the iteration as ONE hipGraph."""
+    `capture()` / `replay()` run the iteration as ONE hipGraph.
+
+    distill=(temperature, alpha): the speaker learns from a teacher (vocab.distill_loss); the batch also holds what
+    `Speaker.teacher_targets` of the teacher gave for it, `teacher_ids` / `teacher_values` [B * Lw, k] and (optionally) `teacher_rest`
+    [B * Lw]."""
 
     rollout_wgrads = False
+    _TEACHER = ("teacher_ids", "teacher_values", "teacher_rest")
 
     def __init__(self, dev, dtype, *, enc=None, dec=None, vocab=992, wemb=256, rnn=512, feature_size=2176, angle_size=128,
-                 drop=0.6, feat_drop=0.3, lr=1e-4, clip_norm=CLIP, graph=False):
-        self.dev, self.dtype = dev, dtype
+                 drop=0.6, feat_drop=0.3, lr=1e-4, clip_norm=CLIP, graph=False, distill=None):
+        self.dev, self.dtype, self.distill = dev, dtype, distill
         self.enc = enc if enc is not None else SpeakerEncoder(feature_size, rnn, drop, True, angle_size, feat_drop, compute_dtype=dtype).to(dev).train()
         self.dec = dec if dec is not None else SpeakerDecoder(vocab, wemb, 0, rnn, drop, compute_dtype=dtype).to(dev).train()
         self.speaker = Speaker(self.enc, self.dec)
@@ -653,7 +658,7 @@ class SpeakerIteration(_GraphedIteration):
             self.live = {k: (v.clone() if torch.is_tensor(v) else v) for k, v in batch.items()}
             self.live["ctx_mask"] = mask
             return self.live
-        for k in ("can", "img", "insts"):
+        for k in ("can", "img", "insts", *(k for k in self._TEACHER if k in self.live)):
             self.live[k].copy_(batch[k], non_blocking=True)
         self.live["lengths"] = batch["lengths"]
         self.live["ctx_mask"].copy_(mask, non_blocking=True)
@@ -668,10 +673,16 @@ class SpeakerIteration(_GraphedIteration):
         with rollout_wgrads(False):                               # (parameter gradients added into .grad by the launches themselves)
             return self._iteration()
 
+    def _targets(self, b):
+        if self.distill is None:
+            return None
+        T, alpha = self.distill
+        return vocab.DistillTargets(b["teacher_ids"], b["teacher_values"], b.get("teacher_rest"), T, alpha)
+
     def _eager(self, b):
         self.opt_e.zero_grad(); self.opt_d.zero_grad()
         # the feature dropout works in place (units.py:322,331): a training loop hands over fresh feature tensors every batch
-        loss = self.speaker.teacher_forcing(b["can"].clone(), b["img"].clone(), b["lengths"], b["insts"], train=True)
+        loss = self.speaker.teacher_forcing(b["can"].clone(), b["img"].clone(), b["lengths"], b["insts"], train=True, distill=self._targets(b))
         loss.backward()
         self.opt_e.step(); self.opt_d.step()
         return loss
@@ -681,7 +692,8 @@ class SpeakerIteration(_GraphedIteration):
         if self.clock is not None:
             self.clock.tick()
         self.opt_e.zero_grad(); self.opt_d.zero_grad()
-        loss = self.speaker.teacher_forcing(b["can"].clone(), b["img"].clone(), b["lengths"], b["insts"], train=True, ctx_mask=b["ctx_mask"])
+        loss = self.speaker.teacher_forcing(b["can"].clone(), b["img"].clone(), b["lengths"], b["insts"], train=True, ctx_mask=b["ctx_mask"],
+                                            distill=self._targets(b))
         loss.backward()
         self.opt_e.step(); self.opt_d.step()
         return loss

@@ -10,7 +10,8 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
-from typing import Optional, Union
+from dataclasses import dataclass
+from typing import Callable, Optional, Union
 
 import torch
 
@@ -249,6 +250,38 @@ def _word_list(a, lists, ids, lens, N, dev, name, size):
             lists.append(lens)
 
 
+@dataclass
+class WordConstraints:
+    """The constraints of a whole decoding loop (`Speaker.infer_batch(constraints=...)`): constrain_logits' arguments, applied to every word
+    with the words so far as the history.  allowed: mask rows (`pack_allowed`); next_rows(t, words [N, t] int64 on the device) -> int64 [N]
+    on the device, each row's mask row for word t -- a grammar's state; None: mask row n (or the only one) throughout."""
+    repetition: Union[float, torch.Tensor] = 1.0
+    presence: Union[float, torch.Tensor] = 0.0
+    frequency: Union[float, torch.Tensor] = 0.0
+    prompt: Optional[torch.Tensor] = None
+    prompt_lengths: Optional[torch.Tensor] = None
+    bias_ids: Optional[torch.Tensor] = None
+    bias_values: Optional[torch.Tensor] = None
+    allowed: Optional[torch.Tensor] = None
+    next_rows: Optional[Callable[[int, torch.Tensor], torch.Tensor]] = None
+
+    def banning(self, word: int, N: int, device) -> "WordConstraints":
+        """The same constraints with one more word banned (a bias of -inf)."""
+        ids = torch.full((N, 1), int(word), dtype=torch.int64, device=device)
+        values = torch.full((N, 1), float("-inf"), device=device)
+        if self.bias_ids is not None:
+            ids = torch.cat((self.bias_ids.expand(N, -1), ids), 1)
+            values = torch.cat((self.bias_values.expand(N, -1), values), 1)
+        return WordConstraints(self.repetition, self.presence, self.frequency, self.prompt, self.prompt_lengths, ids, values, self.allowed, self.next_rows)
+
+    def apply(self, logits: torch.Tensor, words: torch.Tensor) -> torch.Tensor:
+        """constrain_logits for the word after `words` [N, t]."""
+        rows = self.next_rows(words.shape[1], words) if self.next_rows is not None else None
+        return constrain_logits(logits, history=words, prompt=self.prompt, prompt_lengths=self.prompt_lengths, repetition=self.repetition,
+                                presence=self.presence, frequency=self.frequency, bias_ids=self.bias_ids, bias_values=self.bias_values,
+                                allowed=self.allowed, allowed_rows=rows)
+
+
 # ---- a teacher's top logits ------------------------------------------------------------------------------------------------------
 def _temperature(T, who):
     T = float(T)
@@ -288,6 +321,16 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
         _launch(_lib.load().vln_top_logits, "vln_top_logits", dev, z.data_ptr(), max(z.stride(0), V), code, N, V, k, T, values.data_ptr(),
                 ids.data_ptr(), rest.data_ptr(), ws.data_ptr() if nb else None, nb)
     return values, ids, rest
+
+
+@dataclass
+class DistillTargets:
+    """What a teacher leaves for its student (`Speaker.teacher_targets`): top_logits' results for every row and the loss's settings."""
+    ids: torch.Tensor
+    values: torch.Tensor
+    rest: Optional[torch.Tensor] = None
+    temperature: float = 1.0
+    alpha: float = 0.5
 
 
 # ---- distillation ----------------------------------------------------------------------------------------------------------------
