@@ -78,11 +78,15 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
     return x & all;
   };
   // What the counting needs is asked for first (loads come back in order), then the mask bits, then the logits.
-  constexpr int HP = 8;
+  constexpr int HP = 8, PP = 2;
+  const int64_t* prompt = a.prompt + (int64_t)b * a.ld_prompt;
   const int64_t* hist = a.history + (int64_t)b * a.ld_history;
   int64_t first_ids[HP];
 #pragma unroll
   for (int t = 0; t < HP; ++t) first_ids[t] = t * kCThreads + tid < a.H ? hist[t * kCThreads + tid] : -1;
+  int64_t prompt_ids[PP];
+#pragma unroll
+  for (int t = 0; t < PP; ++t) prompt_ids[t] = t * kCThreads + tid < a.P ? prompt[t * kCThreads + tid] : -1;
   int64_t bias_id = -1;
   float bias_val = 0.f;
   if (!BWD && tid < a.n_bias) {
@@ -137,7 +141,15 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
     }
   };
   each(hist, HP * kCThreads, hl, [&](int s) { Cn::count(lds, s); });
-  if (a.P) each(a.prompt + (int64_t)b * a.ld_prompt, 0, length(a.prompt_len, a.P), [&](int s) { Cn::flag(lds, s, Cn::kPrompt); });
+  if (a.P) {
+    const int pl = length(a.prompt_len, a.P);
+#pragma unroll
+    for (int t = 0; t < PP; ++t) {
+      const int s = t * kCThreads + tid < pl ? slot(prompt_ids[t]) : -1;
+      if (s >= 0) Cn::flag(lds, s, Cn::kPrompt);
+    }
+    each(prompt, PP * kCThreads, pl, [&](int s) { Cn::flag(lds, s, Cn::kPrompt); });
+  }
   // The segment's bias entries: slot, entry, value and the logit as it is before any of this row is written (in-place calls).
   int4* bias = reinterpret_cast<int4*>(lds + nwords);
   if (!BWD) {
@@ -148,9 +160,10 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
       }
       const int s = slot(bias_id);
       if (s >= 0) {
-        const float z = (bits_at((int)bias_id) & 1u) ? Elt<E>::ld(in + bias_id) : -INFINITY;
-        bias[atomicAdd(&n_here, 1)] = make_int4(s, j, __float_as_int(bias_val), __float_as_int(z));
+        const float z = Elt<E>::ld(in + bias_id);
+        const unsigned may = bits_at((int)bias_id) & 1u;                   // (a banned word's entry: slot with the top bit set)
         if (Cn::flag(lds, s, Cn::kBias)) n_twice = 1;
+        bias[atomicAdd(&n_here, 1)] = make_int4(may ? s : s | (int)0x80000000, j, __float_as_int(bias_val), __float_as_int(z));
       }
     }
   }
@@ -187,10 +200,10 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
           prev = next;
         }
       }
-      const int s = me.x;
+      const int s = me.x & 0x7fffffff;
       b_col[t] = s < nslot_v ? col0 + s : (s < nslot_v + VEC ? s - nslot_v : g.tail0() + s - nslot_v - VEC);
       b_out[t] = penalised<CT>(__int_as_float(me.w), Cn::get(lds, s), q) + sum;
-      if (!(bits_at(b_col[t]) & 1u)) b_out[t] = -INFINITY;
+      if (me.x < 0) b_out[t] = -INFINITY;
     }
   }
   const float banned = BWD ? 0.f : -INFINITY;

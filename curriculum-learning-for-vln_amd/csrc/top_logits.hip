@@ -171,7 +171,7 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
       most = max(most, gm[i]);
       least = min(least, gm[i] - 1u);          // (0 - 1: an empty group)
     }
-    unsigned th = 0u;                          // fewer groups than k: every element is a candidate
+    unsigned th = 0u;                          // fewer groups than k: no bound
     if (groups >= a.k)
       th = bisect_near(wave_umin(least) + 1u, wave_umax(most), a.k, a.k + a.k / 8 + 2, 12, [&](unsigned b) {
         int c = 0;
@@ -183,7 +183,7 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   }
   __syncthreads();
   unsigned border = bound;                     // candidates reach it: !(x <= tval), tval just below (below +0 comes -0, which compares equal)
-  const float tval = border == 0u ? __builtin_nanf("") : order_value(border == 0x80000000u ? border - 2 : border - 1);
+  const float tval = border == 0u ? 0.f : order_value(border == 0x80000000u ? border - 2 : border - 1);
   constexpr unsigned kNegInf = 0x007fffffu;    // order bits of -inf
   int len = 0;                                 // this wave's list
   uint2* list = reinterpret_cast<uint2*>(cand) + w * CAP;
@@ -196,7 +196,7 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   if (!(fabsf(ref) < 1e30f)) ref = 0.f;
   const float nm = -ref * a.c, cut_off = fmaf(ref, a.c, nm);
   constexpr int UV = 8 / VEC;                  // vectors of 8 elements
-  bool full = border == kNegInf;
+  bool full = border == kNegInf || border == 0u;      // (0: fewer groups than k)
   while (!full) {
     len = 0;
     float sum = 0.f;
@@ -214,21 +214,33 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
 #pragma unroll
       for (int j = 1; j < 8; ++j) mx = nan_max(mx, x[j]);
       if (__ballot(!(mx <= tval))) {
-        int mine = 0, total;
-        bool in[8];
+        auto column = [&](int j) { return g.head + (i + j / VEC * T) * VEC + j % VEC; };
+        if (W == 1) {                          // short rows: most elements of a unit have a candidate in some lane -- one scan places them all
+          int mine = 0, total;
+          bool in[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          in[j] = !(x[j] <= tval) && i + j / VEC * T < v1;
-          mine += in[j] ? 1 : 0;
-        }
-        int at = len - mine + wave_scan(mine, total);
-        len += total;
+          for (int j = 0; j < 8; ++j) { in[j] = !(x[j] <= tval); mine += in[j] ? 1 : 0; }
+          int at = len - mine + wave_scan(mine, total);
+          len += total;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (in[j]) {
-            if (at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), g.head + (i + j / VEC * T) * VEC + j % VEC);
-            ++at;
-            x[j] = -INFINITY;
+          for (int j = 0; j < 8; ++j) {
+            if (in[j]) {
+              if (at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), column(j));
+              ++at;
+              x[j] = -INFINITY;
+            }
+          }
+        } else {                               // long rows: one or two elements of the unit
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool in = !(x[j] <= tval);
+            const u64 mask = __ballot(in);
+            if (mask) {
+              const int at = len + lanes_below(mask);
+              if (in && at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), column(j));
+              x[j] = in ? -INFINITY : x[j];
+              len += __popcll(mask);
+            }
           }
         }
       }
