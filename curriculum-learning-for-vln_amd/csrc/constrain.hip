@@ -77,7 +77,14 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
     if (sh + VEC > 32 && w < last_word) x |= mk[w + 1] << (32 - sh);
     return x & all;
   };
-  // What the counting needs is asked for first (loads come back in order), then the mask bits, then the logits.
+  // Loads come back in order: the mask bits first, which say what logits are needed, then what the counting needs, then the logits.
+  unsigned ok[VPT];
+  uint4 raw[VPT];
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {
+    const int i = v0 + u * kCThreads + tid;
+    ok[u] = i < v1 ? bits_at(g.head + i * VEC) : 0u;
+  }
   constexpr int HP = 8, PP = 2;
   const int64_t* prompt = a.prompt + (int64_t)b * a.ld_prompt;
   const int64_t* hist = a.history + (int64_t)b * a.ld_history;
@@ -92,13 +99,6 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
   if (!BWD && tid < a.n_bias) {
     bias_id = a.bias_ids[(int64_t)b * a.ld_bias_ids + tid];
     bias_val = a.bias_values[(int64_t)b * a.ld_bias_values + tid];
-  }
-  unsigned ok[VPT];
-  uint4 raw[VPT];
-#pragma unroll
-  for (int u = 0; u < VPT; ++u) {
-    const int i = v0 + u * kCThreads + tid;
-    ok[u] = i < v1 ? bits_at(g.head + i * VEC) : 0u;
   }
 #pragma unroll
   for (int u = 0; u < VPT; ++u) {
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kCThreads, 4) __attribute__((amdgpu_num_sgpr(96))) 
     if (s >= 0) Cn::count(lds, s);
   }
   auto each = [&](const int64_t* row, int from, int len, auto&& f) {      // the ids that fall into this segment
-    for (int i = from + tid; i < len; i += 4 * kCThreads) {
+    for (int64_t i = from + tid; i < len; i += 4 * kCThreads) {
       int64_t id[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) id[t] = i + t * kCThreads < len ? row[i + t * kCThreads] : -1;

@@ -14,6 +14,7 @@ from dataclasses import dataclass
 from typing import Callable, Optional, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, losses, ops
 
@@ -122,6 +123,7 @@ class _Constrain(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         logits = ctx.saved_tensors[0]
         N, V = logits.shape
@@ -215,8 +217,8 @@ def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = 
         out = torch.empty(z.shape, dtype=z.dtype, device=dev)
         _constrain_call(z, out, None, a, dev)
         return out
-    if learns or out.requires_grad:
-        raise ValueError("constrain_logits: out= carries no gradient; leave it out, or call it under torch.no_grad() on detached logits")
+    if learns or out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("constrain_logits: out= carries no gradient; leave it out, or call under torch.no_grad()")
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
         raise ValueError(f"constrain_logits: out must be {tuple(logits.shape)} {logits.dtype} on {dev}")
     if N and (_dense(logits, N, V) is not logits or _dense(out, N, V) is not out):
@@ -229,6 +231,7 @@ def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = 
     _gpu(logits, "constrain_logits")
     if N:
         _constrain_call(logits, out, None, a, dev)
+        torch.autograd.graph.increment_version(out)          # (a graph that saved `out` must not use it as if it were unchanged)
     return out
 
 
@@ -370,6 +373,7 @@ class _Distill(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss):
         ctx.saved_tensors
         a, (z, _buf, inv) = ctx.args, ctx.keep
@@ -394,8 +398,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_values
     as two outcomes that share it.
 
     target [N] int64: needed for alpha < 1.  Rows whose target is `ignore_index` -- without targets, rows whose teacher has no mass --
-    have loss and gradient 0 and do not count in the mean (no row counted: nan); a target outside [0, V) otherwise makes its row nan.
-    With targets, a row whose teacher has no mass keeps its hard term.  A student that gives no mass to a word the teacher does has loss
+    have loss and gradient 0 and do not count in the mean (no row counted: nan); with alpha < 1 any other target outside [0, V) makes its
+    row nan.  With targets, a row whose teacher has no mass keeps its hard term.  A student that gives no mass to a word the teacher does has loss
     inf there.  reduction: "mean" over the counted rows, "sum" or "none" ([N]).
 
     One pass over the logits forward, one backward (logits in, gradient out); nothing of size [N, V] is kept in between.  Gradients go

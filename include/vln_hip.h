@@ -388,8 +388,8 @@ int vln_top_logits(const void* logits, int64_t ld, int type, int N, int V, int k
  *   d row / d z_v = alpha T (p_v - sum of q_j with id_j = v)  for a kept word,  alpha T (p_v - r p_v / p_rest)  for any other,
  *                   + (1 - alpha) (softmax(z)_v - [v = target])
  * A word listed twice: two outcomes that share a word.  A row whose target is ignore_index -- without targets, a row whose teacher has
- * no mass -- has loss 0 and gradient 0 and is not counted by the mean (no row counted: NaN); any other target outside [0, V) makes its
- * row NaN.  With targets, a row whose teacher has no mass keeps its hard term.  alpha < 1 needs targets.
+ * no mass -- has loss 0 and gradient 0 and is not counted by the mean (no row counted: NaN); with alpha < 1 any other target outside
+ * [0, V) makes its row NaN.  With targets, a row whose teacher has no mass keeps its hard term.  alpha < 1 needs targets.
  * rows [N] receives the row losses, stats [N, VLN_DISTILL_STATS] (16-byte aligned) what the backward needs; with a reduction, loss [1]
  * and the factor inv_count [1] that the backward takes.  ws: vln_distill_ws_bytes (0: may be NULL), 16-byte aligned. */
 #define VLN_DISTILL_MAX 256

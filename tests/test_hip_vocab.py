@@ -670,3 +670,75 @@ def test_upstream_gradients_and_repeated_backward(vocab):
     assert torch.equal(two, 2 * one)
     rows = vocab.distill_loss(leaf, *args, reduction="none")
     assert torch.equal(torch.autograd.grad(rows.sum(), leaf)[0], one)
+
+
+def test_calls_that_autograd_must_refuse(vocab):
+    """A list or a target changed in place between forward and backward, logits overwritten through out= while a graph holds them, and a second
+    derivative: errors, not wrong numbers."""
+    z, ids, tv, rest, target = distill_case(5, 300, 6, "fp32", 4, True)
+    leaf = z.to(dev()).requires_grad_(True)
+    ids, tv = ids.to(dev()), tv.to(dev())
+    loss = vocab.distill_loss(leaf, ids, tv)
+    ids.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, leaf)
+    hist = torch.zeros(5, 4, dtype=torch.int64, device=dev())
+    out = vocab.constrain_logits(leaf, history=hist, repetition=2.0)
+    hist[0, 0] = 3
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out.sum(), leaf)
+    w = (leaf * 1.0)
+    y = (w * w).sum()                              # the product's backward needs w
+    with torch.no_grad():
+        vocab.constrain_logits(w, history=hist, repetition=2.0, out=w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaf)
+    loss = vocab.distill_loss(leaf, ids, tv)
+    g, = torch.autograd.grad(loss, leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaf)
+
+
+def test_rows_far_apart(vocab):
+    """Rows whose offsets pass 2^31 elements (and 2^32 bytes): views of one large buffer."""
+    V, ld = 1003, (1 << 30) + 7
+    buf = torch.empty(2 * ld + V, dtype=torch.bfloat16, device=dev())
+    z = buf.as_strided((3, V), (ld, 1))
+    g = torch.Generator().manual_seed(0)
+    zc = torch.randn(3, V, generator=g).to(torch.bfloat16)
+    z.copy_(zc)
+    hist = torch.randint(0, V, (3, 20), generator=g)
+    packed = zc.to(dev())
+    kw = dict(history=hist.to(dev()), repetition=1.5, frequency=0.5)
+    assert torch.equal(vocab.constrain_logits(z, **kw), vocab.constrain_logits(packed, **kw))
+    for a, b in zip(vocab.top_logits(z, 9, 2.0), vocab.top_logits(packed, 9, 2.0)):
+        assert torch.equal(a, b)
+    val, ids = torch.topk(zc.float(), 5, dim=1)
+    res = []
+    for x in (z, packed):
+        leaf = x.detach().requires_grad_(True)
+        loss = vocab.distill_loss(leaf, ids.to(dev()), val.to(dev()))
+        res.append((loss.detach(), torch.autograd.grad(loss, leaf)[0]))
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+    want = vocab.constrain_logits(packed, **kw)
+    vocab.constrain_logits(z, out=z, **kw)
+    assert torch.equal(z, want)
+
+
+def test_on_another_stream(vocab):
+    """Inputs made on one stream, the calls on another that waits for it."""
+    z, ids, tv, rest, target = distill_case(64, 5001, 16, "bf16", 9, True)
+    side = torch.cuda.Stream()
+    leaf = z.to(dev()).requires_grad_(True)
+    args = (ids.to(dev()), tv.to(dev()))
+    want = vocab.distill_loss(leaf, *args, teacher_rest=rest.to(dev()), temperature=2.0)
+    wg, = torch.autograd.grad(want, leaf)
+    top = vocab.top_logits(leaf, 5)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = vocab.distill_loss(leaf, *args, teacher_rest=rest.to(dev()), temperature=2.0)
+        gg, = torch.autograd.grad(got, leaf)
+        top2 = vocab.top_logits(leaf, 5)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(want, got) and torch.equal(wg, gg) and all(torch.equal(a, b) for a, b in zip(top, top2))
