@@ -86,6 +86,19 @@ def _constant(t, name: str):
         raise ValueError(f"{name} gets no gradient: it is a constant here (detach it)")
 
 
+def _held(lists):
+    """The lists a backward will read, with their versions: kept like this, not by save_for_backward, because a call's host time is mostly
+    autograd's (and they are small; the logits, which are not, are saved and freed by autograd).  Tensors of inference mode have no version."""
+    return [(t, None if t.is_inference() else t._version) for t in lists if t is not None]
+
+
+def _unchanged(held):
+    for t, version in held:
+        if version is not None and t._version != version:
+            raise RuntimeError(f"a tensor of shape {tuple(t.shape)} that the backward needs has been modified by an inplace operation "
+                               f"(version {t._version}, expected {version})")
+
+
 # ---- constraints -----------------------------------------------------------------------------------------------------------------
 def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
     """bool [G, V] (True = the word is allowed) -> int32 [G, ceil(V / 32)], word v at bit v % 32 of element v // 32: the mask rows that
@@ -118,19 +131,25 @@ class _Constrain(torch.autograd.Function):
         z = _dense(logits, N, V)
         out = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         _constrain_call(z, out, None, args, z.device)
-        ctx.save_for_backward(logits, *lists)         # (a list changed in place before the backward is an error, not a wrong gradient)
-        ctx.args = args
+        ctx.save_for_backward(logits)
+        ctx.args, ctx.held = args, _held(lists)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        logits = ctx.saved_tensors[0]
+        return _Constrain.second(ctx, dout) if torch.is_grad_enabled() else _Constrain.first(ctx, dout)
+
+    @staticmethod
+    def first(ctx, dout):
+        logits, = ctx.saved_tensors
+        _unchanged(ctx.held)
         N, V = logits.shape
         z, d = _dense(logits, N, V), _dense(dout, N, V)
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         _constrain_call(d, dz, z, ctx.args, z.device)
         return dz, None, None
+
+    second = staticmethod(once_differentiable(first.__func__))       # (create_graph=True: a second derivative is an error)
 
 
 def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, history_lengths: Optional[torch.Tensor] = None,
@@ -345,15 +364,14 @@ def _grad_like(z: torch.Tensor, N: int, V: int):
 
 
 def _distill_forward(z, N, V, code, ids, teacher, rest, target, T, alpha, ignore_index, red):
-    """(loss, the filled-in struct, what it points to besides the inputs): the struct serves the backward as well."""
+    """(loss, the filled-in struct, the buffer it points to, 1 / count's address): all but the loss serve the backward as well."""
     dev = z.device
     # one buffer: the rows' statistics (16-byte aligned), 1 / count, and the rows' losses unless they are the result
     own_rows = N if red else 0
     buf = torch.empty(N * _lib.DISTILL_STATS + 4 + own_rows, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev) if red else torch.empty(N, dtype=torch.float32, device=dev)
-    stats, out = buf.data_ptr(), loss.data_ptr()
+    stats, out, K = buf.data_ptr(), loss.data_ptr(), ids.shape[1]
     inv = stats + 4 * N * _lib.DISTILL_STATS
-    K = ids.shape[1]
     a = _lib.Distill(z.data_ptr(), max(z.stride(0), V), ids.data_ptr(), max(ids.stride(0), K), teacher.data_ptr(), max(teacher.stride(0), K),
                      None if rest is None else rest.data_ptr(), None if target is None else target.data_ptr(), ignore_index,
                      inv + 16 if red else out, stats, T, alpha, code, _TYPES[teacher.dtype], N, V, K, 0)
@@ -361,28 +379,36 @@ def _distill_forward(z, N, V, code, ids, teacher, rest, target, T, alpha, ignore
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     _launch(_lib.load().vln_distill_fwd, "vln_distill_fwd", dev, _byref(a), red, out if red else None, inv if red else None,
             ws.data_ptr() if nb else None, nb)
-    return loss, a, (z, buf, inv if red else None)
+    return loss, a, buf, inv if red else None
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, meta):
-        N, V, _, ids, teacher, rest, target = meta[:7]
-        loss, ctx.args, ctx.keep = _distill_forward(_dense(logits, N, V), *meta)
-        ctx.save_for_backward(logits, ids, teacher, rest, target)     # (one of them changed in place before the backward is an error)
+        z = _dense(logits, meta[0], meta[1])
+        loss, ctx.args, ctx.buf, ctx.inv = _distill_forward(z, *meta)
+        ctx.save_for_backward(z)
+        ctx.held = _held(meta[3:7])
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
-        ctx.saved_tensors
-        a, (z, _buf, inv) = ctx.args, ctx.keep
+        return _Distill.second(ctx, dloss) if torch.is_grad_enabled() else _Distill.first(ctx, dloss)
+
+    @staticmethod
+    def first(ctx, dloss):
+        a, inv = ctx.args, ctx.inv
+        z = _dense(ctx.saved_tensors[0], a.N, a.V)
+        a.logits, a.ld = z.data_ptr(), max(z.stride(0), a.V)          # (a checkpoint or a saved-tensor hook returns another tensor)
+        _unchanged(ctx.held)
         dz = _grad_like(z, a.N, a.V)
         stride = 0
         if inv is None and dloss.stride(0) != 0:
             stride, dloss = 1, dloss.contiguous()
         _launch(_lib.load().vln_distill_bwd, "vln_distill_bwd", z.device, _byref(a), dloss.data_ptr(), stride, inv, dz.data_ptr(), dz.stride(0))
         return dz, None
+
+    second = staticmethod(once_differentiable(first.__func__))       # (create_graph=True: a second derivative is an error)
 
 
 def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_values: torch.Tensor, *, teacher_rest: Optional[torch.Tensor] = None,

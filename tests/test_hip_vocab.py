@@ -742,3 +742,28 @@ def test_on_another_stream(vocab):
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     assert torch.equal(want, got) and torch.equal(wg, gg) and all(torch.equal(a, b) for a, b in zip(top, top2))
+
+
+def test_saved_logits_that_come_back_elsewhere(vocab):
+    """Checkpoints (the chain is run again in the backward) and logits that wait on the CPU: the backward reads the tensor that autograd hands
+    back, not the forward's address.  Teachers from inference mode have no version to compare."""
+    from torch.utils.checkpoint import checkpoint
+    z, ids, tv, rest, target = distill_case(33, 5001, 6, "bf16", 5, True)
+    leaf = z.to(dev()).requires_grad_(True)
+    hist = ids.to(dev())
+    with torch.inference_mode():
+        ids, tv, rest = ids.to(dev()) + 0, tv.to(dev()) * 1, rest.to(dev()) * 1
+
+    def chain(x):
+        y = vocab.constrain_logits(x * 1.0, history=hist, repetition=1.5, frequency=0.1)
+        return vocab.distill_loss(y * 1.0, ids, tv, teacher_rest=rest, temperature=2.0)
+
+    want, = torch.autograd.grad(chain(leaf), leaf)
+    assert bool(want.ne(0).any())
+    loss = checkpoint(chain, leaf, use_reentrant=False)
+    trash = [torch.full((33, 5001), float("nan"), dtype=torch.bfloat16, device=dev()) for _ in range(8)]
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+    with torch.autograd.graph.save_on_cpu():
+        loss = chain(leaf)
+    trash += [torch.full((33, 5001), float("nan"), dtype=torch.bfloat16, device=dev()) for _ in range(8)]
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
