@@ -277,7 +277,9 @@ template <typename E, typename CT, int VPT> static int constrain_launch(const vl
   // once: 512 rows x 131072 bf16, 4096 words of history: see below); with few rows they spread over all.
   k.xcds = a.B >= 64 ? 8 : 1;
   const unsigned lds = (unsigned)(((k.seg_vecs * VEC + 2 * VEC) * sizeof(CT) + 15) / 16 * 16 + lists);
-  const dim3 grid((unsigned)((a.B + k.xcds - 1) / k.xcds * k.xcds * k.n_seg));
+  const int64_t groups = ((int64_t)a.B + k.xcds - 1) / k.xcds * k.xcds * k.n_seg;
+  if (!grid_fits(groups, kCThreads, 1)) { set_error("vln_constrain_logits: too many rows for one launch"); return VLN_ERR_ARG; }
+  const dim3 grid((unsigned)groups);
   if (a.backward) VLN_LAUNCH((constrain_kernel<E, CT, VPT, true>), grid, dim3(kCThreads), lds, st, k);
   else VLN_LAUNCH((constrain_kernel<E, CT, VPT, false>), grid, dim3(kCThreads), lds, st, k);
   VLN_CHECK_LAUNCH("constrain_logits");

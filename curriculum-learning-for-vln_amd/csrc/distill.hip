@@ -507,6 +507,7 @@ static int distill_args(const vln_distill* p, DistillArgs& a, const char* who, b
   a.c = kLog2e / p->temperature; a.invT = 1.f / p->temperature; a.T = p->temperature; a.alpha = p->alpha;
   a.rows = p->rows; a.stats = p->stats;
   distill_split(a.N, a.V, p->type == VLN_F32 ? 4 : 8, &a.W, &a.S, &a.seg_vecs);
+  if (!grid_fits(a.N, 64 * a.W, a.S)) { set_error("%s: too many rows for one launch", who); return VLN_ERR_ARG; }
   return VLN_OK;
 }
 

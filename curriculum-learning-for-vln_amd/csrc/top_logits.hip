@@ -574,6 +574,7 @@ extern "C" int vln_top_logits(const void* logits, int64_t ld, int type, int N, i
   if (k < 1 || k > V || k > VLN_TOP_LOGITS_MAX) { vln::set_error("vln_top_logits: k must be 1 .. min(V, %d)", VLN_TOP_LOGITS_MAX); return VLN_ERR_ARG; }
   if (!(temperature >= VLN_TEMPERATURE_MIN && temperature <= VLN_TEMPERATURE_MAX)) { vln::set_error("vln_top_logits: bad temperature"); return VLN_ERR_ARG; }
   const vln::TopPlan p = vln::top_plan(N, V, k, type == VLN_F32 ? 4 : 8);
+  if (!vln::grid_fits(N, p.S > 1 ? vln::kMergeThreads : 64 * p.W, p.S)) { vln::set_error("vln_top_logits: too many or too long rows for one launch"); return VLN_ERR_ARG; }
   const int64_t need = vln::top_ws(p, N);
   if (need && (!ws || ws_bytes < need)) { vln::set_error("vln_top_logits: workspace too small"); return VLN_ERR_ARG; }
   vln::TopArgs a{};

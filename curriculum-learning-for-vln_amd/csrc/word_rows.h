@@ -7,6 +7,9 @@
 
 namespace vln {
 
+// what one launch takes: fewer than 2^32 threads along x, 65535 workgroups along y
+inline bool grid_fits(int64_t x, int threads, int64_t y) { return x * threads < (int64_t)1 << 32 && y <= 65535; }
+
 // One row seen as  head | nv vectors of 16 bytes | tail : rows of an odd vocabulary start at any element, so the first `head` (< VEC)
 // elements in front of a 16-byte boundary and the last `tail` (< VEC) are taken singly.  Vector i covers columns head + i * VEC ...
 template <typename E> struct RowGeo {

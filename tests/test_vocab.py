@@ -148,3 +148,18 @@ def test_c_abi_refusals(vln):
     for kw in (dict(g=None), dict(gs=2), dict(dz=None), dict(ldz=39)):
         assert distill(True, **kw) == 1, kw
     assert lib.vln_distill_fwd(None, 0, None, None, None, 0, None) == 1
+
+
+def test_more_rows_than_a_launch_takes(vln):
+    """A launch takes fewer than 2^32 threads along x and 65535 workgroups along y: refused before it, with a text."""
+    lib, L = vln._lib.load(), vln._lib
+    p = 4096
+    a = L.Constrain()
+    setattr(a, "in", p)
+    a.out, a.ld_in, a.ld_out, a.B, a.V = p, 8, 8, 1 << 23, 8            # 512 threads a row
+    assert lib.vln_constrain_logits(C.byref(a), None) == 1 and b"too many rows" in lib.vln_last_error_string()
+    assert lib.vln_top_logits(p, 8, 0, 1 << 26, 8, 3, 1.0, p, p, p, None, 0, None) == 1 and b"too many" in lib.vln_last_error_string()
+    assert lib.vln_top_logits(p, 1 << 30, 0, 1, (1 << 31) - 1, 3, 1.0, p, p, p, None, 0, None) == 1        # (ld < V)
+    assert lib.vln_top_logits(p, 1 << 31, 0, 1, (1 << 31) - 1, 3, 1.0, p, p, p, None, 0, None) == 1 and b"too long rows" in lib.vln_last_error_string()
+    d = L.Distill(p, 8, p, 3, p, 3, None, None, -1, p, p, 1.0, 1.0, 0, 0, 1 << 26, 8, 3, 0)                 # 64 threads a row
+    assert lib.vln_distill_fwd(C.byref(d), 0, None, None, None, 0, None) == 1 and b"too many rows" in lib.vln_last_error_string()
