@@ -441,15 +441,17 @@ template <typename E, bool TAIL, bool HARD, int W> __global__ __launch_bounds__(
   if (hard && !bad_y && !y_kept && tid == 0 && here((int)y)) Elt<E>::st(dz + y, grad(Elt<E>::ld(p + y)) - gh);
 }
 
-// Waves and segments per row: one wave for short rows (under 16 KB there is nothing to share), four for long ones -- a row is then read by
-// one workgroup front to back, which the memory serves better than 4 x as many rows at once.  With few rows they are split, but no
-// segment gets under two rounds of the workgroup's loads.
+// Waves and segments per row: one wave for rows under 16 KB (5120 x 992 fp32, forward and backward: 23.9 us; four waves: 32.2), four for
+// long ones -- a row is then read by one workgroup front to back, which the memory serves better than 4 x as many rows at once (8192 x
+// 32000 bf16: 318; one wave: 347; at 16 KB the two meet).  Fewer rows than CUs are cut into segments, one workgroup per CU (64 x 131072
+// bf16: 22 us; not cut: 39), none under two rounds of the workgroup's loads; more would only pay for the join (512 x 32000 bf16: 29; two
+// segments: 33).
 static void distill_split(int N, int V, int vec, int* W, int* S, int* seg_vecs) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
   const int nv = (V + vec - 1) / vec;
   *W = nv >= 1024 ? 4 : 1;
   const int round = 64 * *W * 4;
-  const int want = (16 * cus / *W + N - 1) / N, most = (nv + 2 * round - 1) / (2 * round);
+  const int want = (cus + N - 1) / N, most = (nv + 2 * round - 1) / (2 * round);
   int n = want < most ? want : most;
   const int least = (nv + 32767) / 32768;                     // (a segment's bitmap stays at 32 KB of LDS)
   if (n < least) n = least;

@@ -507,8 +507,13 @@ struct TopPlan {
   int W, NVR, G, S, vps, ks, per;       // waves, vectors per thread, groups per thread; segments, vectors and candidates of one, segments of one merge
   int levels; int count[8];     // segments left after each merge level
 };
-// Short rows (<= 256 vectors) with k <= 64: one wave, no barrier to wait for.  Otherwise four waves and the most vectors per thread (16:
-// 64 KB of a row) that still give every CU two workgroups; more, smaller segments otherwise, at least 4 vectors per thread.
+// Short rows (<= 256 vectors) with k <= 64: one wave, no barrier to wait for (5120 x 992 fp32, k 8: 10.6 us; four waves: 22.5).  Rows of up
+// to 64 KB: four waves and the fewest vectors per thread that hold the row -- with few rows too, where segments would occupy more of the
+// chip but their merge is a second launch (us, one segment | segments of 16 KB: 64 x 32000 bf16, k 32: 12.2 | 14.6; 1 x 32000: 9.0 |
+// 10.1; 4096 x 32000, k 64: 83 | 137).  Longer rows are cut: into 64 KB where that gives every CU two workgroups (512 x 50000 bf16, k 32:
+// 28.3; 16 KB: 31.4), into 16 KB where it does not (64 x 50000, k 1: 11.4; 64 KB: 14.3).
+// Groups per thread: one maximum of a thread's vectors is cheaper than four (4096 x 32000, k 16: 71 us; 79), but k has to stay well below
+// the number of maxima, or too much reaches the bound (4096 x 32000, k 256: 1537; 133).
 static TopPlan top_plan(int N, int V, int k, int vec) {
   TopPlan p{};
   const long nv = ((long)V + vec - 1) / vec;
@@ -516,7 +521,7 @@ static TopPlan top_plan(int N, int V, int k, int vec) {
   if (nv <= 256 && k <= 64) { p.W = 1; p.NVR = 4; p.G = k <= 16 ? 1 : 4; }
   else {
     p.W = 4; p.NVR = 16; p.G = k <= 64 ? 1 : 4;
-    while (p.NVR > 4 && (nv <= 256L * (p.NVR / 2) || (long)N * ((nv + 256L * p.NVR - 1) / (256L * p.NVR)) < 2L * cus)) p.NVR /= 2;
+    while (p.NVR > 4 && (nv <= 256L * (p.NVR / 2) || (nv > 256L * 16 && (long)N * ((nv + 256L * p.NVR - 1) / (256L * p.NVR)) < 2L * cus))) p.NVR /= 2;
   }
   const long held = 64L * p.W * p.NVR;
   p.S = (int)((nv + held - 1) / held);
