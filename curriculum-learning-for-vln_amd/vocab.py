@@ -165,7 +165,7 @@ def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = 
         t += the word's `bias_values`;  words that `allowed` bans: -inf
 
     history [N, H] / prompt [N, P]: int64 word ids, any row stride (a slice of the words so far), valid up to *_lengths [N] int64 (None:
-    all); ids outside [0, V) -- padding: -1 -- stand for no word.  repetition (> 0) / presence / frequency: a number, or float32 [N].
+    all); ids outside [0, V) -- padding: -1 -- stand for no word.  repetition (> 0, not subnormal) / presence / frequency: a number, or float32 [N].
     bias_ids int64 / bias_values float32: [N, n] or [n] for every row, n <= 2048; a word listed twice gets both.  allowed: int32 mask
     rows [G, ceil(V / 32)] from `pack_allowed`; allowed_rows int64 [N] picks each row's (-1: unconstrained; anything else outside [0, G)
     bans every word, which is visible, never a read out of range); without it G is N, or 1 for all.  A row whose mask allows nothing is
@@ -193,7 +193,7 @@ def constrain_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = 
             lists.append(v)
         else:
             v = float(v)
-            if not abs(v) < float("inf") or name == "repetition" and v <= 0.0:
+            if not abs(v) < float("inf") or name == "repetition" and v < 2.0 ** -126:
                 raise ValueError(f"constrain_logits: {name} = {v}")
             setattr(a, name + "_all", v)
     if (bias_ids is None) != (bias_values is None):

@@ -352,7 +352,7 @@ int vln_masked_ce_mean_bwd(const float* probs, const int64_t* target, const floa
  * allowed[r * ld_allowed + v / 32], 1 = allowed; the row's mask row is allowed_rows[b] (-1: every word allowed; outside [-1, G): none),
  * without allowed_rows it is b (G == B) or 0 (G == 1).  out may be `in` itself (same stride), otherwise they must not overlap.
  * backward != 0: in = d out, out = d logits (may be the same array), `logits` = the forward's input; biases and penalties get no gradient.
- * repetition / presence / frequency: [B], or NULL and the *_all value. */
+ * repetition (positive, not subnormal) / presence / frequency: [B], or NULL and the *_all value. */
 typedef struct vln_constrain {
   const void* in; void* out; const void* logits;
   int64_t ld_in, ld_out, ld_logits;

@@ -767,3 +767,20 @@ def test_saved_logits_that_come_back_elsewhere(vocab):
         loss = chain(leaf)
     trash += [torch.full((33, 5001), float("nan"), dtype=torch.bfloat16, device=dev()) for _ in range(8)]
     assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+
+
+def test_repetition_divides_like_a_division(vocab):
+    """fp32, one repeated word in every row, penalties and logits over the whole range: the quotient's bits are a division's wherever it is a
+    normal number; an overflow and infinite logits stay infinite."""
+    g = torch.Generator().manual_seed(3)
+    N = 4000
+    r = torch.exp2(torch.rand(N, generator=g) * 240 - 120)
+    z = torch.exp2(torch.rand(N, 1, generator=g) * 240 - 120)
+    r[:1000], z[:1000] = torch.rand(1000, generator=g) + 1.0, torch.rand(1000, 1, generator=g) * 20       # the usual ones
+    r[1000:1004] = torch.tensor([2.0 ** -126, 3.4e38, 1.0, 0.5])
+    z[1000:1004, 0], z[1004, 0] = 3.4e38, float("inf")
+    want = z[:, 0] / r
+    got = vocab.constrain_logits(z.to(dev()), history=torch.zeros(N, 1, dtype=torch.int64, device=dev()), repetition=r.to(dev()))[:, 0].cpu()
+    ok = (want >= 2.0 ** -126) | torch.isinf(want)
+    assert int(ok.sum()) > 3000 and torch.equal(got[ok], want[ok])
+    assert bool((got[~ok] <= 2.0 ** -126).all())
