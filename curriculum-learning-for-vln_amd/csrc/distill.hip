@@ -8,6 +8,11 @@
 // keep (a bitmap of the kept ones in LDS, one byte tested per 8 logits): the mass of the others is a sum of positive terms, never
 // 1 - (sum of the kept), which cancels when the student is sure.  The kept words (<= VLN_DISTILL_MAX per row) are handled by their own
 // lanes: loss terms in the forward, and in the backward their gradients overwrite what the streaming loop wrote there.
+//
+// Measured, us, forward / forward and backward: 8192 x 32000 bf16, K 64, T 2, hard targets 117 / 319 (4.5 and 4.9 TB/s of what is moved, a copy:
+// 5.2); 1021 x 50001 bf16 with the rest 29 / 65; 5120 x 992 fp32 with the rest 14.6 / 24.5; 16 x 992: 6.3 / 11.4, of which three launches are
+// most.  The backward reads the logits a second time rather than keep a gradient from the forward: with an upstream gradient of 1 the latter
+// would move a third less, with any other a third more, and [N, V] would stay alive in between.
 #include <type_traits>
 
 #include "word_rows.h"

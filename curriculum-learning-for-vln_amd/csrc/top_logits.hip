@@ -13,6 +13,11 @@
 // fewer words allowed than asked for), the elements above the bound and, in index order, as many equal to it as are missing are taken
 // (their places from a scan of the counts); only if those above are too many as well is the border itself searched by bisection.
 // Segments leave their candidates, and one workgroup per row selects among them.
+//
+// Measured, us: 4096 rows x 32000 bf16 71 with k 16, 84 with k 64 (3.1 TB/s), 133 with k 256; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.4, of
+// which a launch is most; 4 x 131072 fp32, k 128: 20 (two launches).  Many rows are bound by instructions, not by bytes: two per element for
+// the maxima and about five for the sweep -- unpack, maximum, multiply-add, exponential, sum -- on 4 waves per SIMD.  A wave that streams a row
+// with a running bound (no registers to hold it) takes 120 - 145 us for 4096 x 32000.  Fully masked rows, 64 x 32000, k 1: 12.
 #include "word_rows.h"
 #include "../../include/vln_hip.h"
 

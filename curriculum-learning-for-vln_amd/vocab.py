@@ -276,7 +276,8 @@ def _word_list(a, lists, ids, lens, N, dev, name, size):
 class WordConstraints:
     """The constraints of a whole decoding loop (`Speaker.infer_batch(constraints=...)`): constrain_logits' arguments, applied to every word
     with the words so far as the history.  allowed: mask rows (`pack_allowed`); next_rows(t, words [N, t] int64 on the device) -> int64 [N]
-    on the device, each row's mask row for word t -- a grammar's state; None: mask row n (or the only one) throughout."""
+    on the device, each row's mask row for word t -- a grammar's state; None: mask row n (or the only one) throughout.  infer_batch adds one
+    bias (<UNK>), so that at most 2047 are left."""
     repetition: Union[float, torch.Tensor] = 1.0
     presence: Union[float, torch.Tensor] = 0.0
     frequency: Union[float, torch.Tensor] = 0.0
