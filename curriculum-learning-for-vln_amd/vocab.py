@@ -99,6 +99,14 @@ def _unchanged(held):
                                f"(version {t._version}, expected {version})")
 
 
+def _returned(ctx, N: int, V: int, code: int, device):
+    """The forward's logits as autograd hands them back: a checkpoint or a saved-tensor hook returns another tensor, which has to be alike."""
+    z, = ctx.saved_tensors
+    if z.device != device or _TYPES.get(z.dtype) != code or z.dim() != 2 or z.shape[0] != N or z.shape[1] != V:
+        raise RuntimeError(f"the saved logits came back as {tuple(z.shape)} {z.dtype} on {z.device}, they were [{N}, {V}] on {device}")
+    return _dense(z, N, V)
+
+
 # ---- constraints -----------------------------------------------------------------------------------------------------------------
 def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
     """bool [G, V] (True = the word is allowed) -> int32 [G, ceil(V / 32)], word v at bit v % 32 of element v // 32: the mask rows that
@@ -141,12 +149,11 @@ class _Constrain(torch.autograd.Function):
 
     @staticmethod
     def first(ctx, dout):
-        logits, = ctx.saved_tensors
+        a = ctx.args
+        z, d = _returned(ctx, a.B, a.V, a.type, dout.device), _dense(dout, a.B, a.V)
         _unchanged(ctx.held)
-        N, V = logits.shape
-        z, d = _dense(logits, N, V), _dense(dout, N, V)
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        _constrain_call(d, dz, z, ctx.args, z.device)
+        _constrain_call(d, dz, z, a, z.device)
         return dz, None, None
 
     second = staticmethod(once_differentiable(first.__func__))       # (create_graph=True: a second derivative is an error)
@@ -399,8 +406,8 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def first(ctx, dloss):
         a, inv = ctx.args, ctx.inv
-        z = _dense(ctx.saved_tensors[0], a.N, a.V)
-        a.logits, a.ld = z.data_ptr(), max(z.stride(0), a.V)          # (a checkpoint or a saved-tensor hook returns another tensor)
+        z = _returned(ctx, a.N, a.V, a.type, dloss.device)
+        a.logits, a.ld = z.data_ptr(), max(z.stride(0), a.V)
         _unchanged(ctx.held)
         dz = _grad_like(z, a.N, a.V)
         stride = 0

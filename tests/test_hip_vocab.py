@@ -784,3 +784,15 @@ def test_repetition_divides_like_a_division(vocab):
     ok = (want >= 2.0 ** -126) | torch.isinf(want)
     assert int(ok.sum()) > 3000 and torch.equal(got[ok], want[ok])
     assert bool((got[~ok] <= 2.0 ** -126).all())
+
+
+def test_saved_logits_that_come_back_different(vocab):
+    """A hook that returns the saved logits in another type or shape: an error before any launch."""
+    leaf = torch.randn(6, 500, device=dev()).requires_grad_(True)
+    hist, ids, tv = torch.zeros(6, 3, dtype=torch.int64, device=dev()), torch.zeros(6, 1, dtype=torch.int64, device=dev()), torch.zeros(6, 1, device=dev())
+    for back in (lambda t: t.bfloat16(), lambda t: t[:, :100], lambda t: t[0], lambda t: t.cpu()):
+        for call in (lambda: vocab.constrain_logits(leaf, history=hist, repetition=2.0).sum(), lambda: vocab.distill_loss(leaf, ids, tv)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: back(t) if t.dim() == 2 and t.shape == leaf.shape else t):
+                loss = call()
+            with pytest.raises(RuntimeError, match="came back"):
+                torch.autograd.grad(loss, leaf)
