@@ -1,23 +1,28 @@
 // The k largest logits of every row, sorted, and the log-mass of all others (vln_top_logits): a teacher's targets for vln_distill_*,
 // and with k = 1 the greedy word.  include/vln_hip.h states the contract.
 //
-// Bound: bytes for many rows (the row is read once, into registers: all its loads are in flight at once), the length of one workgroup's
-// chain for few.  A workgroup of W waves holds a row, or one of S segments of it, as NVR vectors of 16 bytes per thread:
-//   1. the largest element of every thread (G groups per thread, so that there are >= 4 k groups): at least k elements reach the k-th
-//      largest of these group maxima, and hardly more than k do -- a bound that costs a bisection over 64 W G numbers;
-//   2. one sweep over the registers: elements above the bound are candidates (an LDS list), all others go into the running (maximum,
-//      sum) of exp(z / T) -- the others' mass is a sum of positive terms, never a difference;
+// Bound: bytes for many rows (the row is read once), the length of one workgroup's chain for few.  A workgroup of W waves takes a row, or
+// one of S segments of it, as NVR vectors of 16 bytes per thread:
+//   1. as they arrive, the maximum and the sum of exp((z - maximum) / T) of every UNIT of 8 elements -- the exponentials, most of the
+//      arithmetic, run under the loads -- and the largest element of every thread (G groups per thread, so that there are >= 4 k groups): at
+//      least k elements reach the k-th largest of these group maxima, and hardly more than k do -- a bound that costs a bisection over
+//      64 W G numbers;
+//   2. units below the bound are joined: one exponential each.  The few that are not are read again, a lane each: elements above the bound
+//      are candidates (an LDS list), the rest goes into the running (maximum, sum) -- the others' mass is a sum of positive terms, never a
+//      difference;
 //   3. a candidate's place is the number of larger ones; places from k on belong to the others.
+// Short rows and segments of 16 KB stay in registers and are swept there once the bound is known: k is no small part of their units.
 // Elements are ordered by (order-preserving bits of the value, lower index first): all distinct, so ties fall to the lowest index and the
 // order in which candidates were collected does not show.  Where more reach the bound than a list holds, or the bound is -inf (rows with
 // fewer words allowed than asked for), the elements above the bound and, in index order, as many equal to it as are missing are taken
 // (their places from a scan of the counts); only if those above are too many as well is the border itself searched by bisection.
 // Segments leave their candidates, and one workgroup per row selects among them.
 //
-// Measured, us: 4096 rows x 32000 bf16 71 with k 16, 84 with k 64 (3.1 TB/s), 133 with k 256; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.4, of
-// which a launch is most; 4 x 131072 fp32, k 128: 20 (two launches).  Many rows are bound by instructions, not by bytes: two per element for
-// the maxima and about five for the sweep -- unpack, maximum, multiply-add, exponential, sum -- on 4 waves per SIMD.  A wave that streams a row
-// with a running bound (no registers to hold it) takes 120 - 145 us for 4096 x 32000.  Fully masked rows, 64 x 32000, k 1: 12.
+// Measured, us: 4096 rows x 32000 bf16 58 with k 16, 60 with k 64 (4.4 TB/s; loads and bound alone 51, a copy's rate), 100 with k 256;
+// 8192 x 4000 bf16, k 16: 22; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.5, of which a launch is most; 4 x 131072 fp32, k 128: 19.5 (two
+// launches).  With rows held in registers until the bound is known 4096 x 32000, k 64, takes 85: every element's exponential, 25 us of
+// instructions, then comes after the loads.  Tried: the next row's loads issued from that sweep, 115 (spilled registers); a wave per row that
+// streams with a running bound, 120 - 145.
 #include "word_rows.h"
 #include "../../include/vln_hip.h"
 
@@ -125,12 +130,12 @@ __device__ __forceinline__ float log_mass(float m, float s, float invT) {
   return s == 0.f ? -INFINITY : (m == INFINITY ? INFINITY : m * invT + logf(s));
 }
 
-// workgroups per CU that the registers are limited to: 4 waves per SIMD hold 64 KB rows, 8 the smaller ones
-template <int W, int NVR> constexpr int row_groups() { return (NVR == 16 ? 4 : NVR == 8 ? 6 : 7) * 4 / W; }
-
-template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W, (row_groups<W, NVR>())) void top_row_kernel(TopArgs a) {
+// (waves per SIMD that the registers are limited to)
+template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W, NVR == 16 ? 5 : W == 1 && NVR == 4 ? 7 : 8) void top_row_kernel(TopArgs a) {
   constexpr int VEC = RowGeo<E>::VEC, T = 64 * W, CAP = VLN_TOP_LOGITS_MAX, GU = NVR / G;      // CAP: candidates of a wave
   __shared__ alignas(16) u64 cand[W * CAP];                   // (first: {value bits, column}, a list per wave)
+  constexpr bool STREAM = NVR > 4;
+  __shared__ unsigned short dirty[STREAM ? W * CAP : 1];      // units to be looked at again, a list per wave
   __shared__ int place[T];
   __shared__ unsigned gmax[T * G];
   __shared__ int counts[W], redo, part[2][W], gt_n[W], eq_n[NVR * W];
@@ -141,25 +146,53 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   const E* p = static_cast<const E*>(a.logits) + n * a.ld;
   const RowGeo<E> g(p, a.V);
   const int v0 = min(g.nv, s * a.vps), v1 = min(g.nv, v0 + a.vps);
-  uint4 raw[NVR];
+  constexpr unsigned none = sizeof(E) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf elements
+  auto ask = [&](int u) {
+    uint4 r = make_uint4(none, none, none, none);
+    if (v0 + u * T + tid < v1) r = ld_vec<E>(p + g.head + (int64_t)(v0 + u * T + tid) * VEC);
+    return r;
+  };
+  constexpr int UV = 8 / VEC, NU = NVR / UV;   // units of 8 elements: vectors of one, units of a thread
+  constexpr int HELD = NVR > 8 ? 8 : NVR;      // vectors in registers at once
+  uint4 raw[HELD];
 #pragma unroll
-  for (int u = 0; u < NVR; ++u) {
-    constexpr unsigned none = sizeof(E) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf elements
-    raw[u] = make_uint4(none, none, none, none);
-    if (v0 + u * T + tid < v1) raw[u] = ld_vec<E>(p + g.head + (int64_t)(v0 + u * T + tid) * VEC);
-  }
+  for (int u = 0; u < HELD; ++u) raw[u] = ask(u);
   // the single elements in front of the first and behind the last vector: threads of the first segment
   int scol = -1;
   if (s == 0) scol = tid < g.head ? tid : (tid >= VEC && tid - VEC < g.tail ? g.tail0() + tid - VEC : -1);
   const float sx = scol >= 0 ? Elt<E>::ld(p + scol) : -INFINITY;
   if (tid == 0) redo = 0;
   float tmax = sx;
+  float um[STREAM ? NU : 1], us[STREAM ? NU : 1];
+  if constexpr (STREAM) {                      // maximum and sum of every unit, as it arrives
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      float x[8];
+#pragma unroll
+      for (int h = 0; h < UV; ++h) {
+        unpack16<E>(raw[(u * UV + h) % HELD], x + h * VEC);
+        if (u * UV + h + HELD < NVR) raw[(u * UV + h) % HELD] = ask(u * UV + h + HELD);
+      }
+      float m = -FLT_MAX, t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, x[i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += exp2_hw((x[i] - m) * a.c);
+      um[u] = m; us[u] = t;
+    }
+  }
 #pragma unroll
   for (int q = 0; q < G; ++q) {
-    VecMax<E> m;
+    float t = -INFINITY;
+    if constexpr (STREAM) {
 #pragma unroll
-    for (int u = q * GU; u < (q + 1) * GU; ++u) m.add(raw[u]);
-    float t = m.get();
+      for (int u = q * (NU / G); u < (q + 1) * (NU / G); ++u) t = fmaxf(t, us[u] == 0.f ? -INFINITY : um[u]);
+    } else {
+      VecMax<E> m;
+#pragma unroll
+      for (int u = q * GU; u < (q + 1) * GU; ++u) m.add(raw[u]);
+      t = m.get();
+    }
     bool has = v0 + q * GU * T + tid < v1;
     if (q == 0 && scol >= 0) { t = fmaxf(t, sx); has = true; }
     tmax = fmaxf(tmax, t);
@@ -192,7 +225,7 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   constexpr unsigned kNegInf = 0x007fffffu;    // order bits of -inf
   int len = 0;                                 // this wave's list
   uint2* list = reinterpret_cast<uint2*>(cand) + w * CAP;
-  // The others' sum.  Every element that is no candidate is at most ref = min(the thread's largest, the bound), so the exponentials are
+  // The others' sum (rows in registers).  Every element that is no candidate is at most ref = min(the thread's largest, the bound), so the exponentials are
   // taken relative to ref, one fused multiply-add each (the rounding of ref * c is taken out again at the end).  Where that is no good
   // reference -- not finite, or everything below it underflows -- the sweep is repeated with a running maximum (`slow`).
   OnlineSum others;
@@ -200,9 +233,71 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   bool slow = __ballot(!(fabsf(ref) < 1e30f) && ref != -INFINITY) != 0, redone = false;
   if (!(fabsf(ref) < 1e30f)) ref = 0.f;
   const float nm = -ref * a.c, cut_off = fmaf(ref, a.c, nm);
-  constexpr int UV = 8 / VEC;                  // vectors of 8 elements
   bool full = border == kNegInf || border == 0u;      // (0: fewer groups than k)
-  while (!full) {
+  if constexpr (STREAM) {
+   if (!full) {
+    // Units that hold a candidate, or whose sum is none (infinities, NaN), are looked at again, a lane each; the others' sums are joined.
+    int n_dirty = 0;
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const bool d = us[u] != 0.f && !(um[u] <= tval && us[u] <= 8.f);
+      const u64 mask = __ballot(d);
+      if (mask) {
+        const int at = n_dirty + lanes_below(mask);
+        if (d && at < CAP) dirty[w * CAP + at] = (unsigned short)(u * T + tid);
+        n_dirty += __popcll(mask);
+      }
+      if (d) { um[u] = -FLT_MAX; us[u] = 0.f; }
+      top = fmaxf(top, um[u]);
+    }
+    others.m = top;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) others.s += us[u] * exp2_hw((um[u] - top) * a.c);
+    wave_sync();
+    for (int j = lane; j - lane < min(n_dirty, CAP); j += 64) {
+      int at = -1;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = -INFINITY;
+      if (j < n_dirty) {
+        at = dirty[w * CAP + j];
+#pragma unroll
+        for (int h = 0; h < UV; ++h) {
+          const int i = v0 + (at / T * UV + h) * T + at % T;
+          if (i < v1) unpack16<E>(ld_vec<E>(p + g.head + (int64_t)i * VEC), x + h * VEC);
+        }
+      }
+      int mine = 0, total;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += !(x[i] <= tval) ? 1 : 0;
+      int to = len - mine + wave_scan(mine, total);
+      len += total;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!(x[i] <= tval)) {
+          if (to < CAP) list[to] = make_uint2(__float_as_uint(x[i]), g.head + (v0 + (at / T * UV + i / VEC) * T + at % T) * VEC + i % VEC);
+          ++to;
+          x[i] = -INFINITY;
+        }
+      }
+      others.add(x, a.c);
+    }
+    if (n_dirty > CAP) len = CAP + 1;          // (the rare forms)
+    if (s == 0) {
+      const bool in = scol >= 0 && !(sx <= tval);
+      int total;
+      const int at = len - 1 + wave_scan(in ? 1 : 0, total);
+      len += total;
+      if (in) { if (at < CAP) list[at] = make_uint2(__float_as_uint(sx), scol); }
+      else if (scol >= 0) others.add1(sx, a.c);
+    }
+    if (lane == 0) counts[w] = len;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) full = full || counts[i] > CAP;
+   }
+  } else while (!full) {
     len = 0;
     float sum = 0.f;
 #pragma unroll
@@ -220,32 +315,19 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
       for (int j = 1; j < 8; ++j) mx = nan_max(mx, x[j]);
       if (__ballot(!(mx <= tval))) {
         auto column = [&](int j) { return g.head + (i + j / VEC * T) * VEC + j % VEC; };
-        if (W == 1) {                          // short rows: most elements of a unit have a candidate in some lane -- one scan places them all
-          int mine = 0, total;
-          bool in[8];
+        // most units of a wave have a candidate in some lane: one scan places them all
+        int mine = 0, total;
+        bool in[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) { in[j] = !(x[j] <= tval); mine += in[j] ? 1 : 0; }
-          int at = len - mine + wave_scan(mine, total);
-          len += total;
+        for (int j = 0; j < 8; ++j) { in[j] = !(x[j] <= tval); mine += in[j] ? 1 : 0; }
+        int at = len - mine + wave_scan(mine, total);
+        len += total;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (in[j]) {
-              if (at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), column(j));
-              ++at;
-              x[j] = -INFINITY;
-            }
-          }
-        } else {                               // long rows: one or two elements of the unit
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const bool in = !(x[j] <= tval);
-            const u64 mask = __ballot(in);
-            if (mask) {
-              const int at = len + lanes_below(mask);
-              if (in && at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), column(j));
-              x[j] = in ? -INFINITY : x[j];
-              len += __popcll(mask);
-            }
+        for (int j = 0; j < 8; ++j) {
+          if (in[j]) {
+            if (at < CAP) list[at] = make_uint2(__float_as_uint(x[j]), column(j));
+            ++at;
+            x[j] = -INFINITY;
           }
         }
       }
@@ -512,22 +594,30 @@ struct TopPlan {
   int W, NVR, G, S, vps, ks, per;       // waves, vectors per thread, groups per thread; segments, vectors and candidates of one, segments of one merge
   int levels; int count[8];     // segments left after each merge level
 };
-// Short rows (<= 256 vectors) with k <= 64: one wave, no barrier to wait for (5120 x 992 fp32, k 8: 10.6 us; four waves: 22.5).  Rows of up
-// to 64 KB: four waves and the fewest vectors per thread that hold the row -- with few rows too, where segments would occupy more of the
-// chip but their merge is a second launch (us, one segment | segments of 16 KB: 64 x 32000 bf16, k 32: 12.2 | 14.6; 1 x 32000: 9.0 |
-// 10.1; 4096 x 32000, k 64: 83 | 137).  Longer rows are cut: into 64 KB where that gives every CU two workgroups (512 x 50000 bf16, k 32:
-// 28.3; 16 KB: 31.4), into 16 KB where it does not (64 x 50000, k 1: 11.4; 64 KB: 14.3).
-// Groups per thread: one maximum of a thread's vectors is cheaper than four (4096 x 32000, k 16: 71 us; 79), but k has to stay well below
-// the number of maxima, or too much reaches the bound (4096 x 32000, k 256: 1537; 133).
+// One wave holds a row of up to 256 vectors (k <= 64) in its registers: no barrier to wait for (5120 x 992 fp32, k 8: 10.6 us; four waves: 22.5;
+// k 1 | 64: 8.4 | 17, as units: 9.1 | 21).  One wave that keeps units takes up to 512 (8192 x 4000 bf16, k 16: 22 us; two waves 25 - 31, four
+// 40), two waves up to 1024 (k <= 128; 8192 x 8000 bf16, k 32: 35; four: 43), four waves the rest: rows of up to 64 KB whole, with the fewest
+// vectors per thread that hold them -- with few rows too, where segments would occupy more of the chip but their merge is a second launch
+// (64 x 32000 bf16, k 1, whole | in segments of 16 KB: 8 | 11; 300 x 16000, k 32: 10 | 18).  Longer rows are cut: into 64 KB where that
+// gives every CU two workgroups (1024 x 50000 bf16, k 32: 44; 16 KB: 52), into 16 KB where it does not (64 x 50000, k 1: 11; 64 KB: 14).
+// Segments of 16 KB stay in registers: units only pay where there are many more of them than k (2000 x 992 fp32, k 128: 21 us; as units: 49;
+// 64 x 50000 fp32, k 256: 25 | 36), and so do rows that have fewer than 4 k units.
+// Groups per thread: one maximum of a thread's vectors is cheaper than four (8192 x 4000, k 16, two waves: 25 us; 30), but k has to stay well below
+// the number of maxima, or too much reaches the bound (4096 x 32000, k 256, in registers: 1537; 133).
 static TopPlan top_plan(int N, int V, int k, int vec) {
   TopPlan p{};
   const long nv = ((long)V + vec - 1) / vec;
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  if (nv <= 256 && k <= 64) { p.W = 1; p.NVR = 4; p.G = k <= 16 ? 1 : 4; }
+  auto units = [&](int vectors) { return (nv < vectors ? nv : vectors) * vec / 8 >= 4 * k; };      // enough of them for k
+  if (nv <= 256 && k <= 64) { p.W = 1; p.NVR = 4; }
+  else if (nv <= 512 && k <= 64 && units(512)) { p.W = 1; p.NVR = 8; }
+  else if (nv <= 1024 && k <= 128 && units(1024)) { p.W = 2; p.NVR = 8; }
   else {
-    p.W = 4; p.NVR = 16; p.G = k <= 64 ? 1 : 4;
+    p.W = 4; p.NVR = 16;
     while (p.NVR > 4 && (nv <= 256L * (p.NVR / 2) || (nv > 256L * 16 && (long)N * ((nv + 256L * p.NVR - 1) / (256L * p.NVR)) < 2L * cus))) p.NVR /= 2;
   }
+  if (p.NVR > 4 && !units(64 * p.W * p.NVR)) p.NVR = 4;
+  p.G = 4 * k <= 64 * p.W ? 1 : 4;
   const long held = 64L * p.W * p.NVR;
   p.S = (int)((nv + held - 1) / held);
   p.vps = (int)((nv + p.S - 1) / p.S);      // equal ones: a short last segment would have too few maxima for a bound
@@ -555,7 +645,9 @@ template <typename E> static int top_launch(TopArgs a, const TopPlan& p, char* w
   };
   a.S = p.S; a.ks = p.ks; a.vps = p.vps;
   if (a.S > 1) take(a.S);
-  if (p.W == 1) top_rows<E, 1, 4>(a, p.G, st);
+  if (p.W == 1 && p.NVR == 4) top_rows<E, 1, 4>(a, p.G, st);
+  else if (p.W == 1) top_rows<E, 1, 8>(a, p.G, st);
+  else if (p.W == 2) top_rows<E, 2, 8>(a, p.G, st);
   else if (p.NVR == 4) top_rows<E, 4, 4>(a, p.G, st);
   else if (p.NVR == 8) top_rows<E, 4, 8>(a, p.G, st);
   else top_rows<E, 4, 16>(a, p.G, st);

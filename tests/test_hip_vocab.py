@@ -796,3 +796,30 @@ def test_saved_logits_that_come_back_different(vocab):
                 loss = call()
             with pytest.raises(RuntimeError, match="came back"):
                 torch.autograd.grad(loss, leaf)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("V,k", [(1100, 1), (2100, 16), (4001, 64), (4001, 65), (7000, 16), (7000, 128), (16001, 32), (31001, 64), (31001, 256), (65001, 40)])
+def test_top_logits_of_unlike_units(vocab, V, k, dt):
+    """Row lengths between the forms (registers of one wave, units of one, two and four waves, whole and cut), and rows in which a few units
+    of eight hold what decides: one word far above all others, runs of large words, infinities and NaN beside ordinary words, words left
+    by a mask of -inf or of the type's lowest value, rows that fall and rise."""
+    t = DT[dt]
+    g = torch.Generator().manual_seed(V + k)
+    z = torch.randn(12, V, generator=g)
+    z[1, V // 3] = 200.0
+    z[2, V // 2:V // 2 + 2 * k] += 30.0
+    z[3, 8 * (torch.randperm(V // 8, generator=g)[:min(k, 3)])] = float("inf")
+    z[4, torch.randperm(V, generator=g)[:min(k, 3)]] = float("nan")
+    z[5, torch.rand(V, generator=g) < 0.98] = NINF
+    z[6, torch.rand(V, generator=g) < 0.98] = torch.finfo(t).min
+    z[7] = torch.linspace(-30, 30, V)
+    z[8] = torch.linspace(30, -30, V)
+    z[9, 5:] = -90.0 + z[9, 5:]
+    z[10] = torch.where(torch.arange(V) % 8 == 3, z[10].abs() + 5, z[10] - 50)       # the largest of every unit in one place
+    z[11, :V - 3] = NINF
+    z = z.to(t)
+    others = z[torch.arange(12) != 4]
+    for T, how in ((1.0, "plain"), (0.05, "odd"), (40.0, "wide")):
+        check_top(vocab, others, k, T, how)
+        check_top(vocab, z[4:5], k, T, how)
