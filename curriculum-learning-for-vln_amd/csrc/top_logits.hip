@@ -19,7 +19,7 @@
 // Segments leave their candidates, and one workgroup per row selects among them.
 //
 // Measured, us: 4096 rows x 32000 bf16 58 with k 16, 60 with k 64 (4.4 TB/s; loads and bound alone 51, a copy's rate), 100 with k 256;
-// 8192 x 4000 bf16, k 16: 22; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.5, of which a launch is most; 4 x 131072 fp32, k 128: 19.5 (two
+// 8192 x 4000 bf16, k 16: 22; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.5, of which a launch is most; 4 x 131072 fp32, k 128: 17.7 (two
 // launches).  With rows held in registers until the bound is known 4096 x 32000, k 64, takes 85: every element's exponential, 25 us of
 // instructions, then comes after the loads.  Tried: the next row's loads issued from that sweep, 115 (spilled registers); a wave per row that
 // streams with a running bound, 120 - 145.
@@ -498,10 +498,10 @@ template <typename E, int W, int NVR, int G> __global__ __launch_bounds__(64 * W
   }
 }
 
-// One workgroup selects the k best of up to `per` segments' candidates, all of them in registers: a bound that at least k reach by
-// bisection over the order bits (one barrier per step), which stops as soon as no more than kMergeList do; these are then placed by rank.
-// Only where that many are equal is the border searched among the indices too.  A row with more segments is merged in levels: blockIdx.y
-// is the group, its result one segment of the next level (last level: the row's result).
+// One workgroup selects the k best of up to `per` segments' candidates, all of them in registers.  The bound again comes from the threads'
+// largest, searched by one wave; what reaches it is placed by rank.  Only if that is more than a list holds do all waves search on among the
+// candidates themselves (a barrier per step), and only where that many are equal among the indices too.  A row with more segments is merged
+// in levels: blockIdx.y is the group, its result one segment of the next level (last level: the row's result).
 constexpr int kMergeThreads = 512, kMergeRegs = 16, kMergeMax = kMergeThreads * kMergeRegs, kMergeList = 512;
 
 template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge_kernel(TopArgs a, int per, u64* keys_out, float2* sums_out) {
@@ -509,7 +509,7 @@ template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge
   __shared__ alignas(16) u64 cand[kMergeList];
   __shared__ int place[kMergeThreads];
   __shared__ int part[2][W];
-  __shared__ unsigned ends[2][W];
+  __shared__ unsigned tops[kMergeThreads], ends[2];
   __shared__ float2 sums[W];
   const long n = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, s0 = blockIdx.y * per, segs = min(per, a.S - s0), total = segs * a.ks;
@@ -519,7 +519,7 @@ template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge
     const float2 o = a.sums[n * a.S + s0 + i];
     others.merge(o.x, o.y, a.c);
   }
-  unsigned hi[kMergeRegs], lo[kMergeRegs], least = 0xffffffffu, most = 0;
+  unsigned hi[kMergeRegs], lo[kMergeRegs], most = 0u;
   const int regs = (total + kMergeThreads - 1) / kMergeThreads;
 #pragma unroll
   for (int i = 0; i < kMergeRegs; ++i) {
@@ -527,13 +527,33 @@ template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge
     const u64 v = i < regs && at < total ? keys[at] : 0ull;
     hi[i] = (unsigned)(v >> 32); lo[i] = (unsigned)v;
     most = max(most, hi[i]);
-    least = min(least, v ? hi[i] : 0xffffffffu);
   }
-  least = wave_umin(least); most = wave_umax(most);
-  if (lane == 0) { ends[0][w] = least; ends[1][w] = most; }
+  tops[tid] = most;
   __syncthreads();
+  if (w == 0) {
+    unsigned gm[W], least = 0xffffffffu;
+    int groups = 0;
+    most = 0u;
 #pragma unroll
-  for (int i = 0; i < W; ++i) { least = min(least, ends[0][i]); most = max(most, ends[1][i]); }
+    for (int i = 0; i < W; ++i) {
+      gm[i] = tops[i * 64 + lane];
+      groups += __popcll(__ballot(gm[i] != 0u));
+      most = max(most, gm[i]);
+      least = min(least, gm[i] - 1u);          // (0 - 1: a thread without any)
+    }
+    most = wave_umax(most);
+    unsigned th = 1u;
+    if (groups >= a.k)
+      th = bisect_near(wave_umin(least) + 1u, most, a.k, a.k + a.k / 8 + 2, 16, [&](unsigned b) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) c += gm[i] >= b ? 1 : 0;
+        return wave_isum(c);
+      });
+    if (lane == 0) { ends[0] = th; ends[1] = most; }
+  }
+  __syncthreads();
+  most = ends[1];
   int turn = 0, before;                       // before: what the waves in front of this one counted
   auto block_count = [&](auto&& has) {
     int c = 0;
@@ -548,11 +568,10 @@ template <typename E> __global__ __launch_bounds__(kMergeThreads) void top_merge
     turn ^= 1;
     return c;
   };
-  unsigned th = 1u, tl = 0u;
-  int nc = block_count([&](unsigned h, unsigned) { return h != 0u; });
-  const int near = min(a.k + a.k / 4 + 32, kMergeList);
-  if (nc > near) {
-    th = bisect_near(least, most, a.k, near, 32, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
+  unsigned th = ends[0], tl = 0u;
+  int nc = block_count([&](unsigned h, unsigned) { return h >= th; });
+  if (nc > kMergeList) {
+    th = bisect_near(th, most, a.k, kMergeList, 32, [&](unsigned t) { return block_count([&](unsigned h, unsigned) { return h >= t; }); });
     nc = block_count([&](unsigned h, unsigned) { return h >= th; });
     if (nc > kMergeList) {
       const int need = a.k - block_count([&](unsigned h, unsigned) { return h > th; });
