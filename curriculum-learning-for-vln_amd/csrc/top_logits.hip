@@ -11,7 +11,7 @@
 //      are candidates (an LDS list), the rest goes into the running (maximum, sum) -- the others' mass is a sum of positive terms, never a
 //      difference;
 //   3. a candidate's place is the number of larger ones; places from k on belong to the others.
-// Short rows and segments of 16 KB stay in registers and are swept there once the bound is known: k is no small part of their units.
+// Short rows stay in registers and are swept there once the bound is known: k is no small part of their units.
 // Elements are ordered by (order-preserving bits of the value, lower index first): all distinct, so ties fall to the lowest index and the
 // order in which candidates were collected does not show.  Where more reach the bound than a list holds, or the bound is -inf (rows with
 // fewer words allowed than asked for), the elements above the bound and, in index order, as many equal to it as are missing are taken
@@ -19,7 +19,7 @@
 // Segments leave their candidates, and one workgroup per row selects among them.
 //
 // Measured, us: 4096 rows x 32000 bf16 58 with k 16, 60 with k 64 (4.4 TB/s; loads and bound alone 51, a copy's rate), 100 with k 256;
-// 8192 x 4000 bf16, k 16: 22; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.5, of which a launch is most; 4 x 131072 fp32, k 128: 17.7 (two
+// 8192 x 4000 bf16, k 16: 22; 5120 x 992 fp32, k 16: 11; 64 x 992, k 1: 4.5, of which a launch is most; 4 x 131072 fp32, k 128: 16.5 (two
 // launches).  With rows held in registers until the bound is known 4096 x 32000, k 64, takes 85: every element's exponential, 25 us of
 // instructions, then comes after the loads.  Tried: the next row's loads issued from that sweep, 115 (spilled registers); a wave per row that
 // streams with a running bound, 120 - 145.
@@ -617,10 +617,11 @@ struct TopPlan {
 // k 1 | 64: 8.4 | 17, as units: 9.1 | 21).  One wave that keeps units takes up to 512 (8192 x 4000 bf16, k 16: 22 us; two waves 25 - 31, four
 // 40), two waves up to 1024 (k <= 128; 8192 x 8000 bf16, k 32: 35; four: 43), four waves the rest: rows of up to 64 KB whole, with the fewest
 // vectors per thread that hold them -- with few rows too, where segments would occupy more of the chip but their merge is a second launch
-// (64 x 32000 bf16, k 1, whole | in segments of 16 KB: 8 | 11; 300 x 16000, k 32: 10 | 18).  Longer rows are cut: into 64 KB where that
-// gives every CU two workgroups (1024 x 50000 bf16, k 32: 44; 16 KB: 52), into 16 KB where it does not (64 x 50000, k 1: 11; 64 KB: 14).
-// Segments of 16 KB stay in registers: units only pay where there are many more of them than k (2000 x 992 fp32, k 128: 21 us; as units: 49;
-// 64 x 50000 fp32, k 256: 25 | 36), and so do rows that have fewer than 4 k units.
+// (64 x 32000 bf16, k 1, whole | in segments of 16 KB: 8 | 11; 300 x 16000, k 32: 10 | 18).  Longer rows are cut: into 64 KB where that gives
+// every CU two workgroups (512 x 131072 bf16, k 32: 38.6; 32 KB: 39.3; 16 KB: 53), into 32 KB where it does not (64 x 50000, k 32: 13.6; 64 KB:
+// 14.8; 16 KB: 14.4.  1 x 131072, k 1: 10.5; 12.2; 10.5).
+// Units only pay where there are many more of them than k: rows with fewer than 4 k stay in registers, 16 KB a workgroup (2000 x 992 fp32, k
+// 128: 18 us; as units: 49).
 // Groups per thread: one maximum of a thread's vectors is cheaper than four (8192 x 4000, k 16, two waves: 25 us; 30), but k has to stay well below
 // the number of maxima, or too much reaches the bound (4096 x 32000, k 256, in registers: 1537; 133).
 static TopPlan top_plan(int N, int V, int k, int vec) {
@@ -633,7 +634,8 @@ static TopPlan top_plan(int N, int V, int k, int vec) {
   else if (nv <= 1024 && k <= 128 && units(1024)) { p.W = 2; p.NVR = 8; }
   else {
     p.W = 4; p.NVR = 16;
-    while (p.NVR > 4 && (nv <= 256L * (p.NVR / 2) || (nv > 256L * 16 && (long)N * ((nv + 256L * p.NVR - 1) / (256L * p.NVR)) < 2L * cus))) p.NVR /= 2;
+    while (p.NVR > 4 && nv <= 256L * (p.NVR / 2)) p.NVR /= 2;
+    if (nv > 256L * 16 && (long)N * ((nv + 256L * 16 - 1) / (256L * 16)) < 2L * cus) p.NVR = 8;
   }
   if (p.NVR > 4 && !units(64 * p.W * p.NVR)) p.NVR = 4;
   p.G = 4 * k <= 64 * p.W ? 1 : 4;
